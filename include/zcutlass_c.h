@@ -28,6 +28,10 @@
  *   zcutlass_nvls_reduce_scatter   reduce-scatter over NVLink SHARP
  *   zcutlass_nvls_barrier       the collectives' cross-rank barrier alone
  *   zcutlass_gemm_gather_a      GEMM reading row blocks of A from several buffers
+ *   zcutlass_quantize_fp8       matrices to 8-bit floating point, a scale per 128
+ *   zcutlass_gemm_fp8           product of 8-bit operands with those scales
+ *   zcutlass_sum_rows           column sums from the quantiser's partial sums
+ *   zcutlass_rotary             rotary positions on q and k heads
  *
  * Integer enum values equal the C++ enum values (Status, DType, LayoutKind).
  * Return values of type int that carry a status use zcutlass_status values.
@@ -153,6 +157,101 @@ int zcutlass_gemm_decode_noalloc(int64_t m, int64_t n, int64_t k, const void* A,
                                  const void* B, int64_t ldb, int32_t b_col_major, const void* C,
                                  int64_t ldc, void* D, int64_t ldd, int32_t dtype, float alpha,
                                  float beta, const void* bias, void* stream);
+
+/* Quantisation to 8-bit floating point (no reference counterpart).
+ *
+ * A group is 1 x 128 values of a row of x (block_rows = 1) or a 128 x 128
+ * block (block_rows = 128); the last group of a row or column may be shorter.
+ * Its scale is the smallest power of two s >= 2^-126 with max|x| <= max8 * s
+ * (1 for a group of zeros), max8 = 448 (e4m3) or 57344 (e5m2), and
+ * q = x / s rounded to nearest even. A group holding an infinity or a NaN gets
+ * s = NaN and q = NaN throughout.
+ *
+ * Two results, either of which may be left out (NULL q or qt, not both),
+ * written in one pass over x:
+ *   q  [rows, cols]  rows groups along each row of x; scale element (r, g) at
+ *                    scale[r * scale_row + g * scale_blk]
+ *   qt [cols, rows]  the transpose of x, groups along each row of the
+ *                    transpose (a column of x); element (c, g) of its scales
+ *                    at scale_t[c * scale_t_row + g * scale_t_blk]
+ * With block_rows = 128 the scale index r (c) counts blocks, and both results
+ * hold the same values. ld* are row strides in elements. x may have any
+ * alignment and stride; q and qt any stride >= their width (a multiple of 16
+ * at a 16-byte aligned base is what zcutlass_gemm_fp8 reads fastest). Padding
+ * of q and qt is not written.
+ * `col_sums` (NULL unless qt is written with block_rows = 1): receives
+ * [ceil(rows / 128), cols] 32-bit sums of x over each 128 rows, which
+ * zcutlass_sum_rows adds up (a bias gradient).
+ * x_type: F16, BF16 or F32; q_type: E4M3 or E5M2. Asynchronous on `stream`. */
+typedef struct zcutlass_quantize_desc {
+  int64_t rows, cols, ldx;
+  int32_t x_type, q_type, block_rows, reserved;
+  int64_t ldq, scale_row, scale_blk;
+  int64_t ldqt, scale_t_row, scale_t_blk;
+  void* stream;
+} zcutlass_quantize_desc;
+
+int zcutlass_quantize_fp8(const zcutlass_quantize_desc* desc, const void* x, void* q, float* scale, void* qt,
+                          float* scale_t, float* col_sums);
+
+/* out[c] = sum over r of part[r * cols + c], in row order, rounded once to
+ * out_type (F16, BF16 or F32). */
+int zcutlass_sum_rows(const float* part, int64_t rows, int64_t cols, void* out, int32_t out_type, void* stream);
+
+/* Product of 8-bit operands with a scale for each block of 128 k (no
+ * reference counterpart), accumulated in 32 bits and rounded once:
+ *
+ *   D[m, n] = sum_b a_scale(m, b) * b_scale(n, b) * sum_{k in block b} A[m, k] * B[n, k] + bias[n]
+ *
+ * A [m, k] and B [n, k] are both K-contiguous with row strides lda, ldb
+ * (elements); each is E4M3 or E5M2, D and bias F16, BF16 or F32. a_scale has
+ * an entry per row of A and block; b_scale per row of B (b_scale_rows = 1) or
+ * per 128 rows of B (b_scale_rows = 128); scales are any 32-bit values and
+ * have element strides *_row, *_blk. Operands at 16-byte aligned addresses
+ * with row strides that are multiples of 16 run on the tcgen05 kernels,
+ * others on a slower predicated kernel. m = 0 or n = 0 succeeds without
+ * writes; k = 0 gives D = bias (or 0). Nothing is allocated. */
+typedef struct zcutlass_fp8_gemm_desc {
+  int64_t m, n, k;
+  int64_t lda, ldb, ldd;
+  int32_t a_type, b_type, d_type, b_scale_rows;
+  int64_t a_scale_row, a_scale_blk;
+  int64_t b_scale_row, b_scale_blk;
+  const void* bias;
+  void* stream;
+} zcutlass_fp8_gemm_desc;
+
+int zcutlass_gemm_fp8(const zcutlass_fp8_gemm_desc* desc, const void* A, const float* a_scale, const void* B,
+                      const float* b_scale, void* D);
+
+/* Rotary positions (no reference counterpart) on `tokens` tokens of q and k
+ * heads of one type (F16, BF16 or F32):
+ *
+ *   half layout (interleaved = 0):  pair i of a head = (x[i], x[i + rotary_dim / 2])
+ *   interleaved = 1:                pair i           = (x[2 i], x[2 i + 1])
+ *   (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin); inverse = 1 negates the sines (the gradient)
+ *
+ * computed in 32 bits and rounded once; values rotary_dim..head_dim-1 of a
+ * head are copied. Row p of `table` (row stride table_ld >= rotary_dim) holds
+ * the rotary_dim / 2 cosines and then the sines of position p, for p in
+ * [0, table_rows). A negative position marks padding: its heads are copied as
+ * they are. A position >= table_rows does the same and sets the device error
+ * word (zcutlass_device_error), site 32.
+ * Strides of tokens and heads are in elements, values of a head contiguous;
+ * out may equal in (in place), and must not overlap it otherwise. k_heads = 0:
+ * q only. positions: int32 (positions64 = 0) or int64. */
+typedef struct zcutlass_rotary_desc {
+  int64_t tokens;
+  int32_t q_heads, k_heads, head_dim, rotary_dim;
+  int32_t dtype, interleaved, inverse, positions64;
+  int64_t q_token, q_head, q_out_token, q_out_head;
+  int64_t k_token, k_head, k_out_token, k_out_head;
+  int64_t table_rows, table_ld;
+  void* stream;
+} zcutlass_rotary_desc;
+
+int zcutlass_rotary(const zcutlass_rotary_desc* desc, const void* q, void* q_out, const void* k, void* k_out,
+                    const void* positions, const float* table);
 
 /* Tensor-parallel all-reduce over NVLink SHARP (no reference counterpart: the
  * reference leaves the row-parallel all-reduce to vLLM/NCCL). Sums, in place,

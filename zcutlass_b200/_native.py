@@ -59,6 +59,35 @@ def make_desc(m, n, k, lda, ldb, ldc, ldd, dtype, alpha=1.0, beta=0.0, bias=None
                     alpha, beta, bias, stream, a_layout, b_layout, c_layout, d_layout)
 
 
+class QuantizeDesc(ctypes.Structure):
+    """Field-for-field image of zcutlass_quantize_desc."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "cols", "ldx")] + \
+        [(n, ctypes.c_int32) for n in ("x_type", "q_type", "block_rows", "reserved")] + \
+        [(n, ctypes.c_int64) for n in ("ldq", "scale_row", "scale_blk", "ldqt", "scale_t_row", "scale_t_blk")] + \
+        [("stream", ctypes.c_void_p)]
+
+
+class Fp8GemmDesc(ctypes.Structure):
+    """Field-for-field image of zcutlass_fp8_gemm_desc."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("m", "n", "k", "lda", "ldb", "ldd")] + \
+        [(n, ctypes.c_int32) for n in ("a_type", "b_type", "d_type", "b_scale_rows")] + \
+        [(n, ctypes.c_int64) for n in ("a_scale_row", "a_scale_blk", "b_scale_row", "b_scale_blk")] + \
+        [("bias", ctypes.c_void_p), ("stream", ctypes.c_void_p)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """Field-for-field image of zcutlass_rotary_desc."""
+
+    _fields_ = [("tokens", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in ("q_heads", "k_heads", "head_dim", "rotary_dim", "dtype", "interleaved",
+                                       "inverse", "positions64")] + \
+        [(n, ctypes.c_int64) for n in ("q_token", "q_head", "q_out_token", "q_out_head", "k_token", "k_head",
+                                       "k_out_token", "k_out_head", "table_rows", "table_ld")] + \
+        [("stream", ctypes.c_void_p)]
+
+
 _P = ctypes.POINTER(GemmDesc)
 _v = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -97,6 +126,10 @@ SIGNATURES = {
     "zcutlass_gemm_decode_noalloc": (ctypes.c_int, [_i64, _i64, _i64, _v, _i64, _v, _i64, ctypes.c_int32, _v, _i64,
                                                     _v, _i64, ctypes.c_int32, ctypes.c_float, ctypes.c_float, _v,
                                                     _v]),
+    "zcutlass_quantize_fp8": (ctypes.c_int, [ctypes.POINTER(QuantizeDesc), _v, _v, _v, _v, _v, _v]),
+    "zcutlass_sum_rows": (ctypes.c_int, [_v, _i64, _i64, _v, ctypes.c_int32, _v]),
+    "zcutlass_gemm_fp8": (ctypes.c_int, [ctypes.POINTER(Fp8GemmDesc), _v, _v, _v, _v, _v]),
+    "zcutlass_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryDesc), _v, _v, _v, _v, _v, _v]),
 }
 
 _LIB: ctypes.CDLL | None = None

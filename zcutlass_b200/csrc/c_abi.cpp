@@ -4,9 +4,25 @@
 
 #include "zcutlass/gemm.hpp"
 
+#include <climits>
+
 #include "launchers.hpp"
+#include "layer_ops.hpp"
 
 namespace {
+
+bool float_type(int32_t t) { return t == ZCUTLASS_F16 || t == ZCUTLASS_BF16 || t == ZCUTLASS_F32; }
+bool fp8_type(int32_t t) { return t == ZCUTLASS_E4M3 || t == ZCUTLASS_E5M2; }
+bool aligned_to(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+uintptr_t size_of(int32_t float_dtype) { return float_dtype == ZCUTLASS_F32 ? 4 : 2; }
+
+// Largest extent the kernels index with 32-bit tile coordinates.
+constexpr int64_t kMaxExtent = INT_MAX - 1024;
+
+int status_of(cudaError_t e) {
+  return e == cudaSuccess ? ZCUTLASS_SUCCESS
+                          : (e == cudaErrorInvalidValue ? ZCUTLASS_INVALID_ARGUMENT : ZCUTLASS_RUNTIME_ERROR);
+}
 
 zcutlass::GemmDesc to_desc(const zcutlass_gemm_desc* d) {
   zcutlass::GemmDesc g{d->m,
@@ -148,6 +164,69 @@ int zcutlass_nvls_reduce_scatter(void* mc_ptr, void* local_ptr, int64_t nbytes, 
                                                         rank, world, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? ZCUTLASS_SUCCESS
                           : (e == cudaErrorInvalidValue ? ZCUTLASS_INVALID_ARGUMENT : ZCUTLASS_RUNTIME_ERROR);
+}
+
+int zcutlass_quantize_fp8(const zcutlass_quantize_desc* d, const void* x, void* q, float* scale, void* qt,
+                          float* scale_t, float* col_sums) {
+  if (d == nullptr || d->rows < 0 || d->cols < 0 || d->rows > kMaxExtent || d->cols > kMaxExtent)
+    return ZCUTLASS_INVALID_ARGUMENT;
+  if (!float_type(d->x_type) || !fp8_type(d->q_type)) return ZCUTLASS_NOT_SUPPORTED;
+  if (d->block_rows != 1 && d->block_rows != 128) return ZCUTLASS_NOT_SUPPORTED;
+  if (d->rows == 0 || d->cols == 0) return ZCUTLASS_SUCCESS;
+  if (x == nullptr || (q == nullptr && qt == nullptr)) return ZCUTLASS_INVALID_ARGUMENT;
+  if ((q != nullptr && (scale == nullptr || d->ldq < d->cols)) ||
+      (qt != nullptr && (scale_t == nullptr || d->ldqt < d->rows)) || d->ldx < d->cols)
+    return ZCUTLASS_INVALID_ARGUMENT;
+  if (!aligned_to(x, size_of(d->x_type)) || !aligned_to(scale, 4) || !aligned_to(scale_t, 4) || !aligned_to(col_sums, 4))
+    return ZCUTLASS_INVALID_ARGUMENT;
+  if (col_sums != nullptr && (qt == nullptr || d->block_rows != 1)) return ZCUTLASS_INVALID_ARGUMENT;
+  return status_of(zcb::launch_quantize_fp8(*d, x, q, scale, qt, scale_t, col_sums));
+}
+
+int zcutlass_sum_rows(const float* part, int64_t rows, int64_t cols, void* out, int32_t out_type, void* stream) {
+  if (rows < 0 || cols < 0 || cols > kMaxExtent) return ZCUTLASS_INVALID_ARGUMENT;
+  if (!float_type(out_type)) return ZCUTLASS_NOT_SUPPORTED;
+  if (cols == 0) return ZCUTLASS_SUCCESS;
+  if ((part == nullptr && rows > 0) || out == nullptr || !aligned_to(part, 4) || !aligned_to(out, size_of(out_type)))
+    return ZCUTLASS_INVALID_ARGUMENT;
+  return status_of(zcb::launch_sum_rows(part, rows, cols, out, out_type, static_cast<cudaStream_t>(stream)));
+}
+
+int zcutlass_gemm_fp8(const zcutlass_fp8_gemm_desc* d, const void* A, const float* a_scale, const void* B,
+                      const float* b_scale, void* D) {
+  if (d == nullptr || d->m < 0 || d->n < 0 || d->k < 0) return ZCUTLASS_INVALID_ARGUMENT;
+  if (d->m > kMaxExtent || d->n > kMaxExtent || d->k > kMaxExtent) return ZCUTLASS_INVALID_ARGUMENT;
+  if (!fp8_type(d->a_type) || !fp8_type(d->b_type) || !float_type(d->d_type)) return ZCUTLASS_NOT_SUPPORTED;
+  if (d->b_scale_rows != 1 && d->b_scale_rows != 128) return ZCUTLASS_NOT_SUPPORTED;
+  if (d->m == 0 || d->n == 0) return ZCUTLASS_SUCCESS;
+  if (D == nullptr || d->ldd < d->n) return ZCUTLASS_INVALID_ARGUMENT;
+  if (d->k > 0 && (A == nullptr || B == nullptr || a_scale == nullptr || b_scale == nullptr))
+    return ZCUTLASS_INVALID_ARGUMENT;
+  if (d->lda < d->k || d->ldb < d->k) return ZCUTLASS_INVALID_ARGUMENT;
+  if (!aligned_to(a_scale, 4) || !aligned_to(b_scale, 4) || !aligned_to(D, size_of(d->d_type)) ||
+      !aligned_to(d->bias, size_of(d->d_type)))
+    return ZCUTLASS_INVALID_ARGUMENT;
+  return status_of(zcb::launch_gemm_fp8(*d, A, a_scale, B, b_scale, D));
+}
+
+int zcutlass_rotary(const zcutlass_rotary_desc* d, const void* q, void* q_out, const void* k, void* k_out,
+                    const void* positions, const float* table) {
+  if (d == nullptr || d->tokens < 0 || d->q_heads < 0 || d->k_heads < 0 || d->head_dim < 0 || d->rotary_dim < 0)
+    return ZCUTLASS_INVALID_ARGUMENT;
+  if (!float_type(d->dtype)) return ZCUTLASS_NOT_SUPPORTED;
+  if (d->rotary_dim % 2 != 0 || d->rotary_dim > d->head_dim || d->table_rows < 0 || d->table_ld < d->rotary_dim)
+    return ZCUTLASS_INVALID_ARGUMENT;
+  if (d->head_dim > 65536 || d->q_heads > 65536 || d->k_heads > 65536 || d->tokens > kMaxExtent)
+    return ZCUTLASS_INVALID_ARGUMENT;
+  if (d->tokens == 0 || d->head_dim == 0 || d->q_heads + d->k_heads == 0) return ZCUTLASS_SUCCESS;
+  if ((d->q_heads > 0 && (q == nullptr || q_out == nullptr)) || (d->k_heads > 0 && (k == nullptr || k_out == nullptr)))
+    return ZCUTLASS_INVALID_ARGUMENT;
+  if (positions == nullptr || (d->table_rows > 0 && d->rotary_dim > 0 && table == nullptr)) return ZCUTLASS_INVALID_ARGUMENT;
+  const uintptr_t e = size_of(d->dtype);
+  if (!aligned_to(q, e) || !aligned_to(q_out, e) || !aligned_to(k, e) || !aligned_to(k_out, e) || !aligned_to(table, 4) ||
+      !aligned_to(positions, d->positions64 ? 8 : 4))
+    return ZCUTLASS_INVALID_ARGUMENT;
+  return status_of(zcb::launch_rotary(*d, q, q_out, k, k_out, positions, table));
 }
 
 // For callers that may not allocate device memory at call time (see the

@@ -586,6 +586,8 @@ cudaError_t launch_swapab_km(const LaunchArgs& a, DeviceSlot* slot, int splits) 
 
 }  // namespace
 
+bool programmatic_launch() { return pdl_enabled(); }
+
 const DeviceInfo* current_device_info() {
   DeviceSlot* slot = current_slot();
   return slot ? &slot->info : nullptr;

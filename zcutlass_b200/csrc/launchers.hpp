@@ -42,6 +42,10 @@ struct DeviceInfo {
   int* error_word = nullptr;  // device address of this device's error word
 };
 const DeviceInfo* current_device_info();
+// Whether kernels are launched with programmatic stream serialization
+// (ZCUTLASS_PDL=0 turns it off); such kernels wait for the previous kernel on
+// their stream before their first global memory access.
+bool programmatic_launch();
 
 // Persistent tcgen05 kernel, 128 x bn tiles (bn in {128, 256}).
 cudaError_t launch_umma_gemm(const LaunchArgs& args, int bn);

@@ -10,16 +10,26 @@
 //   torch.ops.zcutlass.linear(x, weight, bias=None) -> y
 //       nn.functional.linear semantics: weight is the PyTorch [N, K] layout and
 //       is consumed directly as a column-major B (no transposed copy).
+//   torch.ops.zcutlass.{quantize_fp8, gemm_fp8, linear_fp8, linear_fp8_forward,
+//       linear_fp8_backward, rotary, rotary_}  8-bit block-scaled linears and
+//       rotary positions over the C ABI (documented in torch_ops.py)
 //
-// This file only adapts tensors to zcutlass::gemm; all kernels live in libzcutlass.so.
+// This file only adapts tensors to the library's entry points; all kernels live in libzcutlass.so.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <optional>
+#include <string_view>
+#include <tuple>
+#include <vector>
 
 #include "zcutlass/gemm.hpp"
+#include "zcutlass_c.h"
 
 namespace {
 
@@ -137,6 +147,294 @@ at::Tensor linear_op(const at::Tensor& x, const at::Tensor& weight,
   return y.view(out_shape);
 }
 
+// ---------------------------------------------------------------- 8-bit linears
+
+void* current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+void check_status(int status, const char* what) {
+  TORCH_CHECK(status == ZCUTLASS_SUCCESS, what, " failed: ", zcutlass_status_to_string(status));
+}
+
+int32_t float_code(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kHalf: return ZCUTLASS_F16;
+    case at::kBFloat16: return ZCUTLASS_BF16;
+    case at::kFloat: return ZCUTLASS_F32;
+    default: TORCH_CHECK(false, name, " must be float16, bfloat16 or float32");
+  }
+}
+
+int32_t fp8_code(at::ScalarType t, const char* name) {
+  TORCH_CHECK(t == at::kFloat8_e4m3fn || t == at::kFloat8_e5m2, name, " must be float8_e4m3fn or float8_e5m2");
+  return t == at::kFloat8_e4m3fn ? ZCUTLASS_E4M3 : ZCUTLASS_E5M2;
+}
+
+constexpr int64_t kFp8Group = 128;
+int64_t groups(int64_t n) { return (n + kFp8Group - 1) / kFp8Group; }
+
+// Row stride of a matrix whose rows are contiguous (one row or no values: any).
+int64_t row_stride(const at::Tensor& t, const char* name) {
+  if (t.numel() == 0) return std::max<int64_t>(t.size(1), 1);
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " must have contiguous rows");
+  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), name, " must not have overlapping rows");
+  return t.size(0) <= 1 ? std::max<int64_t>(t.size(1), 1) : t.stride(0);
+}
+
+// An 8-bit matrix with rows padded to 16 bytes (what TMA can describe).
+at::Tensor empty_fp8(int64_t rows, int64_t cols, at::ScalarType t, const at::Tensor& like) {
+  const int64_t ld = (cols + 15) / 16 * 16;
+  return at::empty({rows, ld}, like.options().dtype(t)).narrow(1, 0, cols);
+}
+
+// Scales [rows, groups], rows contiguous: the product's kernels read the scales of neighbouring rows together.
+at::Tensor empty_row_scales(int64_t rows, int64_t cols, const at::Tensor& like) {
+  return at::empty({groups(cols), rows}, like.options().dtype(at::kFloat)).t();
+}
+
+struct Quantized {
+  at::Tensor q, scale, qt, scale_t, col_sums;
+};
+
+Quantized quantize(const at::Tensor& x, bool rows, bool columns, int64_t block_rows, at::ScalarType type, bool sums) {
+  Quantized r;
+  const int64_t m = x.size(0), n = x.size(1);
+  zcutlass_quantize_desc d{};
+  d.rows = m, d.cols = n, d.ldx = row_stride(x, "x");
+  d.x_type = float_code(x, "x"), d.q_type = fp8_code(type, "dtype"), d.block_rows = static_cast<int32_t>(block_rows);
+  const auto f32 = x.options().dtype(at::kFloat);
+  if (rows) {
+    r.q = empty_fp8(m, n, type, x);
+    r.scale = block_rows == 1 ? empty_row_scales(m, n, x) : at::empty({groups(m), groups(n)}, f32);
+    d.ldq = r.q.stride(0), d.scale_row = r.scale.stride(0), d.scale_blk = r.scale.stride(1);
+  }
+  if (columns) {
+    r.qt = empty_fp8(n, m, type, x);
+    r.scale_t = block_rows == 1 ? empty_row_scales(n, m, x) : at::empty({groups(n), groups(m)}, f32);
+    d.ldqt = r.qt.stride(0), d.scale_t_row = r.scale_t.stride(0), d.scale_t_blk = r.scale_t.stride(1);
+  }
+  if (sums) r.col_sums = at::empty({groups(m), n}, f32);
+  d.stream = current_stream();
+  const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  check_status(zcutlass_quantize_fp8(&d, x.data_ptr(), ptr(r.q), static_cast<float*>(ptr(r.scale)), ptr(r.qt),
+                                     static_cast<float*>(ptr(r.scale_t)), static_cast<float*>(ptr(r.col_sums))),
+               "zcutlass_quantize_fp8");
+  return r;
+}
+
+std::vector<at::Tensor> quantize_fp8_op(const at::Tensor& x, std::string_view layout, std::optional<at::ScalarType> dtype) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a rank-2 CUDA tensor");
+  const at::ScalarType t = dtype.value_or(at::kFloat8_e4m3fn);
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (layout == "rows") {
+    const Quantized r = quantize(x, true, false, 1, t, false);
+    return {r.q, r.scale};
+  }
+  if (layout == "columns") {
+    const Quantized r = quantize(x, false, true, 1, t, false);
+    return {r.qt, r.scale_t};
+  }
+  if (layout == "both") {
+    const Quantized r = quantize(x, true, true, 1, t, false);
+    return {r.q, r.scale, r.qt, r.scale_t};
+  }
+  if (layout == "blocks") {
+    const Quantized r = quantize(x, true, false, kFp8Group, t, false);
+    return {r.q, r.scale};
+  }
+  TORCH_CHECK(layout == "blocks_both", "layout must be rows, columns, both, blocks or blocks_both");
+  const Quantized r = quantize(x, true, true, kFp8Group, t, false);
+  return {r.q, r.scale, r.qt, r.scale_t};
+}
+
+void check_fp8_operand(const at::Tensor& t, const at::Tensor& scale, const char* name, bool blocks_allowed) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2, name, " must be a rank-2 CUDA tensor");
+  (void)fp8_code(t.scalar_type(), name);
+  TORCH_CHECK(scale.is_cuda() && scale.dim() == 2 && scale.scalar_type() == at::kFloat, name,
+              "_scale must be a rank-2 float32 CUDA tensor");
+  TORCH_CHECK(scale.device() == t.device(), name, "_scale must be on the same CUDA device as ", name);
+  const bool per_row = scale.size(0) == t.size(0);
+  const bool per_block = blocks_allowed && scale.size(0) == groups(t.size(0));
+  TORCH_CHECK((per_row || per_block) && scale.size(1) == groups(t.size(1)), name, "_scale must have shape [",
+              blocks_allowed ? "rows or ceil(rows / 128)" : "rows", ", ceil(columns / 128)] of ", name);
+}
+
+at::Tensor run_gemm_fp8(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale,
+                        const std::optional<at::Tensor>& bias, at::ScalarType out_type) {
+  const int64_t m = a.size(0), n = b.size(0), k = a.size(1);
+  at::Tensor d = at::empty({m, n}, a.options().dtype(out_type));
+  zcutlass_fp8_gemm_desc g{};
+  g.m = m, g.n = n, g.k = k;
+  g.lda = row_stride(a, "A"), g.ldb = row_stride(b, "B"), g.ldd = n;
+  g.a_type = fp8_code(a.scalar_type(), "A"), g.b_type = fp8_code(b.scalar_type(), "B");
+  g.d_type = float_code(d, "out_dtype");
+  g.b_scale_rows = b_scale.size(0) == n ? 1 : 128;
+  g.a_scale_row = a_scale.stride(0), g.a_scale_blk = a_scale.stride(1);
+  g.b_scale_row = b_scale.stride(0), g.b_scale_blk = b_scale.stride(1);
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->is_cuda() && bias->device() == a.device() && bias->dim() == 1 && bias->is_contiguous(),
+                "bias must be a contiguous rank-1 CUDA tensor on the operands' device");
+    TORCH_CHECK(bias->scalar_type() == out_type, "bias dtype must match the result's");
+    TORCH_CHECK(bias->size(0) == n, "bias length must equal B.shape[0]");
+    g.bias = bias->data_ptr();
+  }
+  g.stream = current_stream();
+  check_status(zcutlass_gemm_fp8(&g, a.data_ptr(), a_scale.data_ptr<float>(), b.data_ptr(), b_scale.data_ptr<float>(),
+                                 d.data_ptr()),
+               "zcutlass_gemm_fp8");
+  return d;
+}
+
+at::Tensor gemm_fp8_op(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale,
+                       const std::optional<at::Tensor>& bias, std::optional<at::ScalarType> out_dtype) {
+  check_fp8_operand(a, a_scale, "A", false);
+  check_fp8_operand(b, b_scale, "B", true);
+  TORCH_CHECK(a.device() == b.device(), "A and B must be on the same CUDA device");
+  TORCH_CHECK(a.size(1) == b.size(1), "A.shape[1] must equal B.shape[1]");
+  const c10::cuda::CUDAGuard guard(a.device());
+  return run_gemm_fp8(a, a_scale, b, b_scale, bias, out_dtype.value_or(at::kBFloat16));
+}
+
+// x as a matrix [rows, last dimension] of contiguous rows (a copy only where its strides leave no other way).
+at::Tensor as_rows(const at::Tensor& x) {
+  int64_t rows = 1;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+  const at::Tensor x2 = x.reshape({rows, x.size(-1)});
+  const bool ok = (x2.size(1) <= 1 || x2.stride(1) == 1) && (rows <= 1 || x2.stride(0) >= x2.size(1));
+  return ok ? x2 : x2.contiguous();
+}
+
+at::Tensor linear_fp8_op(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
+                         const std::optional<at::Tensor>& bias) {
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 1, "x must be a CUDA tensor");
+  (void)float_code(x, "x");
+  check_fp8_operand(w, w_scale, "weight", true);
+  TORCH_CHECK(x.device() == w.device(), "x and weight must be on the same CUDA device");
+  TORCH_CHECK(x.size(-1) == w.size(1), "x.shape[-1] must equal weight.shape[1]");
+  const c10::cuda::CUDAGuard guard(x.device());
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = w.size(0);
+  const Quantized r = quantize(as_rows(x), true, false, 1, at::kFloat8_e4m3fn, false);
+  return run_gemm_fp8(r.q, r.scale, w, w_scale, bias, x.scalar_type()).view(shape);
+}
+
+// The differentiable linear: y, then what its backward pass needs of x and w, each in 8 bits and
+// transposed (undefined where the gradient it serves is not wanted).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_fp8_forward_op(
+    const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, bool need_dx, bool need_dw) {
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 1, "x must be a CUDA tensor");
+  TORCH_CHECK(w.is_cuda() && w.dim() == 2, "weight must be a rank-2 CUDA tensor");
+  TORCH_CHECK(x.device() == w.device(), "x and weight must be on the same CUDA device");
+  TORCH_CHECK(x.size(-1) == w.size(1), "x.shape[-1] must equal weight.shape[1]");
+  const c10::cuda::CUDAGuard guard(x.device());
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = w.size(0);
+  const Quantized qx = quantize(as_rows(x), true, need_dw, 1, at::kFloat8_e4m3fn, false);
+  const Quantized qw = quantize(as_rows(w), true, need_dx, kFp8Group, at::kFloat8_e4m3fn, false);
+  const at::Tensor y = run_gemm_fp8(qx.q, qx.scale, qw.q, qw.scale, bias, x.scalar_type()).view(shape);
+  const at::Tensor none = at::empty({0}, x.options());
+  return {y, need_dx ? qw.qt : none, need_dx ? qw.scale_t : none, need_dw ? qx.qt : none, need_dw ? qx.scale_t : none};
+}
+
+// dx = Q(dy) Q(w), dw = Q(dy^T) Q(x^T)^T, db = column sums of dy; empty tensors where not wanted.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_fp8_backward_op(
+    const at::Tensor& grad, const at::Tensor& wt, const at::Tensor& wt_scale, const at::Tensor& xt, const at::Tensor& xt_scale,
+    bool need_dx, bool need_dw, bool need_db, at::ScalarType dw_dtype) {
+  TORCH_CHECK(grad.is_cuda() && grad.dim() >= 1, "dy must be a CUDA tensor");
+  const c10::cuda::CUDAGuard guard(grad.device());
+  const at::Tensor dy = as_rows(grad);
+  at::Tensor dx = at::empty({0}, dy.options()), dw = dx, db = dx;
+  if (!need_dx && !need_dw && !need_db) return {dx, dw, db};
+  const Quantized r = quantize(dy, need_dx, need_dw || need_db, 1, at::kFloat8_e4m3fn, need_db);
+  if (need_dx) {
+    check_fp8_operand(wt, wt_scale, "weight", true);
+    std::vector<int64_t> shape(grad.sizes().begin(), grad.sizes().end());
+    shape.back() = wt.size(0);
+    dx = run_gemm_fp8(r.q, r.scale, wt, wt_scale, std::nullopt, dy.scalar_type()).view(shape);
+  }
+  if (need_dw) {
+    check_fp8_operand(xt, xt_scale, "x", true);
+    dw = run_gemm_fp8(r.qt, r.scale_t, xt, xt_scale, std::nullopt, dw_dtype);
+  }
+  if (need_db) {
+    db = at::empty({dy.size(1)}, dy.options());
+    check_status(zcutlass_sum_rows(r.col_sums.data_ptr<float>(), r.col_sums.size(0), dy.size(1), db.data_ptr(),
+                                   float_code(db, "dy"), current_stream()),
+                 "zcutlass_sum_rows");
+  }
+  return {dx, dw, db};
+}
+
+// ---------------------------------------------------------------- rotary positions
+
+void check_heads(const at::Tensor& t, const char* name, const at::Tensor& q) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 3, name, " must be a rank-3 CUDA tensor [tokens, heads, head_dim]");
+  (void)float_code(t, name);
+  TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, name, " must have contiguous heads (last dimension)");
+  TORCH_CHECK(t.scalar_type() == q.scalar_type() && t.device() == q.device() && t.size(0) == q.size(0) &&
+                  t.size(2) == q.size(2),
+              "q and k must match in dtype, device, tokens and head_dim");
+}
+
+void run_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_out, const at::Tensor& k_out,
+                const at::Tensor& positions, const at::Tensor& table, bool interleaved, bool inverse) {
+  check_heads(q, "q", q);
+  check_heads(k, "k", q);
+  TORCH_CHECK(positions.device() == q.device() && table.device() == q.device(),
+              "positions and table must be on the device of q and k");
+  TORCH_CHECK(positions.dim() == 1 && positions.is_contiguous() && positions.size(0) == q.size(0),
+              "positions must be a contiguous rank-1 tensor with one entry per token");
+  TORCH_CHECK(positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt,
+              "positions must be int32 or int64");
+  TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kFloat && (table.size(1) <= 1 || table.stride(1) == 1),
+              "table must be a float32 matrix [positions, rotary_dim] with contiguous rows");
+  TORCH_CHECK(table.size(1) % 2 == 0 && table.size(1) <= q.size(2),
+              "table.shape[1] (the rotary dimension) must be even and no more than the head dimension");
+  zcutlass_rotary_desc d{};
+  d.tokens = q.size(0);
+  d.q_heads = static_cast<int32_t>(q.size(1)), d.k_heads = static_cast<int32_t>(k.size(1));
+  d.head_dim = static_cast<int32_t>(q.size(2)), d.rotary_dim = static_cast<int32_t>(table.size(1));
+  d.dtype = float_code(q, "q"), d.interleaved = interleaved, d.inverse = inverse;
+  d.positions64 = positions.scalar_type() == at::kLong;
+  d.q_token = q.stride(0), d.q_head = q.stride(1), d.q_out_token = q_out.stride(0), d.q_out_head = q_out.stride(1);
+  d.k_token = k.stride(0), d.k_head = k.stride(1), d.k_out_token = k_out.stride(0), d.k_out_head = k_out.stride(1);
+  d.table_rows = table.size(0);
+  d.table_ld = table.size(0) <= 1 ? table.size(1) : table.stride(0);
+  d.stream = current_stream();
+  check_status(zcutlass_rotary(&d, q.data_ptr(), q_out.data_ptr(), k.data_ptr(), k_out.data_ptr(), positions.data_ptr(),
+                               table.data_ptr<float>()),
+               "zcutlass_rotary");
+}
+
+std::tuple<at::Tensor, at::Tensor> rotary_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                                             const at::Tensor& table, bool interleaved, bool inverse) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor q_out = at::empty(q.sizes(), q.options()), k_out = at::empty(k.sizes(), k.options());
+  run_rotary(q, k, q_out, k_out, positions, table, interleaved, inverse);
+  return {q_out, k_out};
+}
+
+void rotary_inplace_op(at::Tensor q, at::Tensor k, const at::Tensor& positions, const at::Tensor& table,
+                       bool interleaved, bool inverse) {
+  at::assert_no_internal_overlap(q);
+  at::assert_no_internal_overlap(k);
+  at::assert_no_overlap(q, k);
+  const c10::cuda::CUDAGuard guard(q.device());
+  run_rotary(q, k, q, k, positions, table, interleaved, inverse);
+}
+
+// While the current stream is being captured: refuses a leaf whose gradient accumulator was made on another
+// stream and is still alive (an eager graph of the same leaf is). The backward pass would wait for that
+// stream, which ends the capture, or the process.
+void check_capture_op(const at::Tensor& leaf) {
+  if (!leaf.requires_grad() || leaf.grad_fn() != nullptr) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (accumulator == nullptr) return;
+  const auto made_on = accumulator->stream();
+  TORCH_CHECK(!made_on.has_value() || *made_on == at::cuda::getCurrentCUDAStream(leaf.get_device()).unwrap(),
+              "a graph of this leaf made on another stream is still alive: drop it (its outputs and losses) before "
+              "capturing a backward pass");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(zcutlass_torch, m) {
@@ -149,10 +447,30 @@ TORCH_LIBRARY(zcutlass, m) {
   m.def("gemm(Tensor A, Tensor B, Tensor? C=None, Tensor? bias=None, float alpha=1.0, float beta=0.0) -> Tensor");
   m.def("gemm_out(Tensor A, Tensor B, Tensor? C, Tensor? bias, float alpha, float beta, Tensor(a!) D) -> ()");
   m.def("linear(Tensor x, Tensor weight, Tensor? bias=None) -> Tensor");
+  m.def("quantize_fp8(Tensor x, str layout=\"rows\", ScalarType? dtype=None) -> Tensor[]");
+  m.def("gemm_fp8(Tensor A, Tensor A_scale, Tensor B, Tensor B_scale, Tensor? bias=None, ScalarType? out_dtype=None) -> Tensor");
+  m.def("linear_fp8(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias=None) -> Tensor");
+  m.def("linear_fp8_forward(Tensor x, Tensor weight, Tensor? bias, bool need_dx, bool need_dw) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_fp8_backward(Tensor dy, Tensor weight_t, Tensor weight_t_scale, Tensor x_t, Tensor x_t_scale, "
+        "bool need_dx, bool need_dw, bool need_db, ScalarType dw_dtype) -> (Tensor, Tensor, Tensor)");
+  m.def("rotary(Tensor q, Tensor k, Tensor positions, Tensor table, bool interleaved=False, bool inverse=False) -> "
+        "(Tensor, Tensor)");
+  m.def("rotary_(Tensor(a!) q, Tensor(b!) k, Tensor positions, Tensor table, bool interleaved=False, "
+        "bool inverse=False) -> ()");
+  m.def("check_capture(Tensor leaf) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(zcutlass, CUDA, m) {
   m.impl("gemm", gemm_op);
   m.impl("gemm_out", gemm_out_op);
   m.impl("linear", linear_op);
+  m.impl("quantize_fp8", quantize_fp8_op);
+  m.impl("gemm_fp8", gemm_fp8_op);
+  m.impl("linear_fp8", linear_fp8_op);
+  m.impl("linear_fp8_forward", linear_fp8_forward_op);
+  m.impl("linear_fp8_backward", linear_fp8_backward_op);
+  m.impl("rotary", rotary_op);
+  m.impl("rotary_", rotary_inplace_op);
+  m.impl("check_capture", check_capture_op);
 }

@@ -5,6 +5,11 @@ Loading registers (CUDA dispatch key only):
     torch.ops.zcutlass.gemm(...)        same op, product namespace
     torch.ops.zcutlass.gemm_out(A, B, C, bias, alpha, beta, D) -> ()
     torch.ops.zcutlass.linear(x, weight[N, K], bias=None) -> y
+    torch.ops.zcutlass.quantize_fp8(x, layout="rows", dtype=None) -> Tensor[]
+    torch.ops.zcutlass.gemm_fp8(A, A_scale, B, B_scale, bias=None, out_dtype=None) -> D
+    torch.ops.zcutlass.linear_fp8(x, weight, weight_scale, bias=None) -> y
+    torch.ops.zcutlass.rotary(q, k, positions, table, interleaved=False, inverse=False) -> (q, k)
+    torch.ops.zcutlass.rotary_(q, k, positions, table, ...) -> ()   in place
 
 `selected_gemm_config` mirrors the reference's extension query
 (python/zcutlass_torch/csrc/zcutlass_torch.cpp:91-149 in supercatking/zcutlass):
@@ -13,6 +18,8 @@ same checks, same dict keys, answered by the C ABI telemetry.
 
 from __future__ import annotations
 
+import functools
+import math
 from pathlib import Path
 
 from . import _native
@@ -126,3 +133,246 @@ def linear(x, weight, bias=None):
 
     load()
     return torch.ops.zcutlass.linear(x, weight, bias)
+
+
+# ---------------------------------------------------------------- 8-bit linears
+
+
+def _no_gradient(name: str, *tensors) -> None:
+    import torch
+
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient: use linear_fp8_train, or call it under torch.no_grad()")
+
+
+def quantize_fp8(x, layout: str = "rows", dtype=None) -> tuple:
+    """x [R, C] (float16, bfloat16 or float32) in 8-bit floating point with a
+    scale per group of 128: x ~= q * scale.
+
+    layout  "rows"         (q [R, C], scale [R, ceil(C / 128)])
+            "columns"      (q [C, R], scale [C, ceil(R / 128)]) of x.T: what a weight gradient reads
+            "both"         the two of "rows", then the two of "columns", in one read of x
+            "blocks"       (q [R, C], scale [ceil(R / 128), ceil(C / 128)]): weights
+            "blocks_both"  the same, then the same values for x.T
+    dtype   torch.float8_e4m3fn (default) or torch.float8_e5m2
+
+    A scale is the smallest power of two (>= 2^-126) that keeps its group
+    within the type's largest value, 1 for a group of zeros; q = x / scale
+    rounded to nearest even. A group with an infinity or a NaN becomes NaN
+    throughout, its scale too. Rows of q are padded to 16 bytes in memory
+    (stride), as gemm_fp8 reads them fastest."""
+    import torch
+
+    load()
+    _no_gradient("quantize_fp8", x)
+    return tuple(torch.ops.zcutlass.quantize_fp8(x, layout, dtype))
+
+
+def gemm_fp8(a, a_scale, b, b_scale, bias=None, out_dtype=None):
+    """a [M, K] @ b [N, K].T (+ bias), both in 8-bit floating point (e4m3 or
+    e5m2, mixed freely), accumulated in 32 bits and rounded once to out_dtype
+    (bfloat16 by default, float16, float32).
+
+    a_scale [M, ceil(K / 128)]; b_scale [N, ceil(K / 128)], or
+    [ceil(N / 128), ceil(K / 128)] for weights in 128 x 128 blocks: float32 of
+    any value and any strides."""
+    import torch
+
+    load()
+    _no_gradient("gemm_fp8", a_scale, b_scale, bias)
+    return torch.ops.zcutlass.gemm_fp8(a, a_scale, b, b_scale, bias, out_dtype)
+
+
+def linear_fp8(x, weight, weight_scale, bias=None):
+    """x [..., K] @ weight [N, K].T (+ bias) with the weight held in 8 bits
+    (quantize_fp8(w, "blocks"), or a checkpoint's values and scales) and x
+    quantised by rows on the way in; y has x's dtype. For serving; training
+    uses linear_fp8_train."""
+    import torch
+
+    load()
+    _no_gradient("linear_fp8", x, weight_scale, bias)
+    return torch.ops.zcutlass.linear_fp8(x, weight, weight_scale, bias)
+
+
+def _check_capture(*tensors) -> None:
+    """Under stream capture: refuses leaves that an eager graph made on another stream still holds, whose
+    backward pass would end the capture (or the process)."""
+    import torch
+
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        for t in tensors:
+            if t is not None and t.is_cuda and t.requires_grad:
+                torch.ops.zcutlass.check_capture(t)
+
+
+@functools.cache
+def _linear_fp8_function():
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    class LinearFp8(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias):
+            need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+            y, *kept = torch.ops.zcutlass.linear_fp8_forward(x, weight, bias, need_dx, need_dw)
+            ctx.save_for_backward(*kept)
+            ctx.weight_dtype = weight.dtype
+            return y
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, dy):
+            need_dx, need_dw, need_db = ctx.needs_input_grad
+            dx, dw, db = torch.ops.zcutlass.linear_fp8_backward(dy, *ctx.saved_tensors, need_dx, need_dw, need_db,
+                                                                ctx.weight_dtype)
+            return dx if need_dx else None, dw if need_dw else None, db if need_db else None
+
+    return LinearFp8
+
+
+def linear_fp8_train(x, weight, bias=None):
+    """x [..., K] @ weight [N, K].T (+ bias) from unquantised operands, with
+    all three products of a training step in 8-bit floating point (e4m3):
+
+        y  = Q(x) Q(w).T + bias     x by rows, w in 128 x 128 blocks
+        dx = Q(dy) Q(w)             dy by rows
+        dw = Q(dy.T) Q(x.T).T       dy and x by columns
+        db = sum of dy over tokens
+
+    each accumulated in 32 bits and rounded once to x's dtype (dw: weight's).
+    x, bias: one of float16, bfloat16, float32; weight: any of them. The
+    backward pass keeps x and weight in 8 bits only. Capturing a step into a
+    CUDA graph is refused while an eager graph of the same leaves is alive."""
+    load()
+    _check_capture(x, weight, bias)
+    return _linear_fp8_function().apply(x, weight, bias)
+
+
+# ---------------------------------------------------------------- rotary positions
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[list[float], float]:
+    """(radians per position of each of the rotary_dim / 2 pairs, factor on
+    cosines and sines). `scaling` stretches positions for long contexts:
+
+        None                                  base^(-2 i / rotary_dim)
+        {"type": "linear", "factor"}          all frequencies / factor
+        {"type": "ntk", "factor"}             base * factor^(rotary_dim / (rotary_dim - 2))
+        {"type": "llama3", "factor", "original", "low": 1, "high": 4}
+            frequencies below `low` turns over the original length / factor,
+            those above `high` turns kept, blended linearly in between
+        {"type": "yarn", "factor", "original", "fast": 32, "slow": 1, "attention": 0.1 ln(factor) + 1}
+            pair indices blended between those that turn `fast` and `slow`
+            times over the original length; cosines and sines * attention"""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and at least 2")
+    half = rotary_dim // 2
+    kind = "none" if scaling is None else scaling.get("type")
+    if kind not in ("none", "linear", "ntk", "llama3", "yarn"):
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    factor = 1.0 if scaling is None else float(scaling["factor"])
+    if not factor > 0 or not base > 0:
+        raise ValueError("base and the scaling factor must be positive")
+    if kind == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("ntk scaling needs a rotary_dim above 2")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = [base ** (-2.0 * i / rotary_dim) for i in range(half)]
+    if kind in ("none", "ntk"):
+        return freq, 1.0
+    if kind == "linear":
+        return [f / factor for f in freq], 1.0
+    original = float(scaling["original"])
+    if not original > 0:
+        raise ValueError("the original length must be positive")
+    if kind == "llama3":
+        low, high = float(scaling.get("low", 1.0)), float(scaling.get("high", 4.0))
+        if not high > low:
+            raise ValueError("llama3 scaling needs high > low")
+        keep = [min(1.0, max(0.0, (original * f / (2 * math.pi) - low) / (high - low))) for f in freq]
+        return [k * f + (1 - k) * f / factor for k, f in zip(keep, freq)], 1.0
+    fast, slow = float(scaling.get("fast", 32.0)), float(scaling.get("slow", 1.0))
+
+    def index(turns: float) -> float:  # the (real) pair index that makes `turns` turns over the original length
+        return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    lo, hi = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rotary_dim - 1)
+    span = max(hi - lo, 1e-3)
+    keep = [1.0 - min(1.0, max(0.0, (i - lo) / span)) for i in range(half)]
+    attention = float(scaling.get("attention", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
+    return [k * f + (1 - k) * f / factor for k, f in zip(keep, freq)], attention
+
+
+def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, scaling: dict | None = None, device=None):
+    """[positions, rotary_dim] float32: the cosines of positions 0..positions-1
+    in the first half of each row, the sines in the second. Angles and their
+    functions are computed in 64 bits, so far positions stay exact. Made once
+    and kept, for any number of layers and calls."""
+    import torch
+
+    freq, factor = rotary_frequencies(rotary_dim, base, scaling)
+    if positions < 1:
+        raise ValueError("positions must be at least 1")
+    f = torch.tensor(freq, dtype=torch.float64, device=device)
+    half = rotary_dim // 2
+    table = torch.empty(positions, rotary_dim, dtype=torch.float32, device=device)
+    for p0 in range(0, positions, 65536):  # bounds the 64-bit temporaries
+        angle = torch.arange(p0, min(p0 + 65536, positions), dtype=torch.float64, device=device)[:, None] * f
+        table[p0:p0 + 65536, :half] = angle.cos() * factor
+        table[p0:p0 + 65536, half:] = angle.sin() * factor
+    return table
+
+
+@functools.cache
+def _rotary_function():
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    class Rotary(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, positions, table, interleaved):
+            ctx.save_for_backward(positions, table)
+            ctx.interleaved = interleaved
+            return torch.ops.zcutlass.rotary(q, k, positions, table, interleaved)
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, dq, dk):
+            positions, table = ctx.saved_tensors
+            dq, dk = (g if g.shape[-1] <= 1 or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk))
+            dq, dk = torch.ops.zcutlass.rotary(dq, dk, positions, table, ctx.interleaved, True)
+            return dq, dk, None, None, None
+
+    return Rotary
+
+
+def rotary(q, k, positions, table, interleaved: bool = False):
+    """Rotary positions on q [tokens, q_heads, head_dim] and k [tokens,
+    k_heads, head_dim] (float16, bfloat16 or float32, any token and head
+    strides, so views of a packed qkv matrix serve); returns new tensors,
+    differentiable in q and k.
+
+    positions: int32 or int64 [tokens]; table: rotary_table(...), whose width
+    is the rotary dimension (at most head_dim; the rest of a head is copied).
+    interleaved: pairs (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2).
+    A negative position marks padding, whose heads are copied as they are. A
+    position at or beyond the table's end does the same and sets the device
+    error word (zcutlass_b200.tp.check_device_error raises on it)."""
+    import torch
+
+    load()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        _check_capture(q, k)
+        return _rotary_function().apply(q, k, positions, table, interleaved)
+    return torch.ops.zcutlass.rotary(q, k, positions, table, interleaved)
+
+
+def rotary_(q, k, positions, table, interleaved: bool = False) -> None:
+    """rotary() in place, without gradients."""
+    import torch
+
+    load()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        raise RuntimeError("rotary_ has no gradient: use rotary, or call it under torch.no_grad()")
+    torch.ops.zcutlass.rotary_(q, k, positions, table, interleaved)

@@ -54,7 +54,8 @@ class TPGroup:
 def check_device_error() -> None:
     """Raises if a kernel of the library recorded an error on the current
     device since the last check (a bounded wait that gave up: an NVLS barrier
-    whose peers never arrived, or a GEMM pipeline wait). After such an error
+    whose peers never arrived, or a GEMM pipeline wait; or a rotary position
+    beyond its table). After such an error
     the outputs of the steps since the last check must not be used: the NVLS
     reduction skips its work once the error word is set. Reading the word
     synchronises the device; call it between steps, not inside a capture."""
@@ -63,6 +64,9 @@ def check_device_error() -> None:
     code = _native.device_error(clear=True)
     if code < 0:
         raise RuntimeError("zcutlass device error word unreadable: the device synchronisation failed")
+    if code >> 4 == 32:
+        raise RuntimeError(f"zcutlass device error word 0x{code:x}: a rotary position lay beyond the end of its table; "
+                           "the heads of that token were left as they were")
     if code != 0:
         raise RuntimeError(f"zcutlass device error word 0x{code:x} (site {code >> 4}, role {code & 15}): "
                            "a bounded wait gave up; the results since the last check are invalid")
