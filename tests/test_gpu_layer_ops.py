@@ -127,6 +127,35 @@ def test_gemm_types(cuda_device, mnk, fa, fb):
     check_gemm(a, sa, b, sb, F16)
 
 
+KERNELS = ["fp8_generic", "fp8_swap16", "fp8_swap32", "fp8_swap64", "fp8_swap128", "fp8_pair"]
+
+
+@pytest.mark.parametrize("b_rows", [False, True], ids=["b_blocks", "b_rows"])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_gemm_every_kernel(cuda_device, monkeypatch, kernel, b_rows):
+    """Each kernel over ragged edges in every dimension, odd and even counts of k blocks, several tiles per
+    CTA, every output type, with and without bias, aligned and odd rows of D."""
+    monkeypatch.setenv("ZCUTLASS_FORCE_KERNEL", kernel)
+    for i, (m, n, k) in enumerate([(1, 1, 1), (16, 128, 128), (17, 200, 300), (130, 264, 1000), (300, 520, 384), (513, 777, 640),
+                                   (256, 512, 1152)]):
+        a, sa, b, sb = operands(m, n, k, b_rows, seed=i)
+        for out in (BF16, F16, F32):
+            check_gemm(a, sa, b, sb, out, rand(n, seed=9, dtype=out) if i % 2 else None)
+    if kernel == "fp8_pair":  # more tiles than CTA pairs, an odd number of blocks
+        a, sa, b, sb = operands(2500, 3000, 640, b_rows)
+        check_gemm(a, sa, b, sb, BF16)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("m", [3, 30, 60, 200])
+def test_gemm_splits(cuda_device, monkeypatch, m, splits):
+    monkeypatch.setenv("ZCUTLASS_SPLITK", str(splits))
+    for n in (256, 333):
+        a, sa, b, sb = operands(m, n, 2100, False)
+        check_gemm(a, sa, b, sb, BF16, rand(n, seed=3, dtype=BF16))
+        check_gemm(a, sa, b, sb, F32)
+
+
 @pytest.mark.parametrize("m", [4, 40, 200, 600])
 def test_gemm_strides(cuda_device, m):
     """Unpadded odd rows and offset bases (no TMA), scales in every stride order, views of larger buffers."""

@@ -1,0 +1,137 @@
+// Parts the 8-bit tcgen05 kernels share: the kind::f8f6f4 MMA, packed 32-bit
+// arithmetic and the scale-and-add that moves one 128-k block's product from
+// TMEM into register accumulators.
+//
+// A scale that changes every 128 k cannot stay inside the tensor core's running
+// sum, and general 32-bit scales cannot be given to it. So each block's product
+// (4 MMAs of k = 32) goes to a TMEM buffer of its own, and the accumulation
+// acc += (sa * sb) * product runs in 32 bits on registers, one TMEM read and one
+// packed fma per two values, while the MMAs of the next blocks fill the other
+// buffers.
+#pragma once
+
+#include "fp8_generic_gemm.cuh"
+#include "sm100_ptx.cuh"
+
+namespace zcb {
+namespace fp8 {
+
+constexpr int kBlockK = 128;  // bytes: one swizzled shared-memory row, one scale
+constexpr int kMmaK = 32;
+
+// Instruction descriptor for kind::f8f6f4 with an f32 accumulator, K-major
+// operands: bits 4-5 D format (1 = f32), 7-9 A and 10-12 B format (0 e4m3,
+// 1 e5m2), 17-22 N>>3, 24-28 M>>4.
+__host__ __device__ constexpr uint32_t idesc(int m, int n, bool a_e5m2, bool b_e5m2) {
+  return (1u << 4) | ((a_e5m2 ? 1u : 0u) << 7) | ((b_e5m2 ? 1u : 0u) << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      " .reg .pred p;\n"
+      " setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      " .reg .pred p;\n"
+      " setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// Waits for the thread's TMEM loads; the registers pass through so that no use of them moves above the wait.
+__device__ __forceinline__ void tmem_ld_wait_x16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+// Two 32-bit values in one register pair.
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  uint32_t lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ uint64_t both(float v) { return pack2(__float_as_uint(v), __float_as_uint(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+// Barrier kId of kThreads threads that also tells every one of them whether all passed true.
+template <int kId, int kThreads>
+__device__ __forceinline__ bool barrier_and(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      " .reg .pred p, q;\n"
+      " setp.ne.b32 p, %3, 0;\n"
+      " barrier.cta.red.and.pred q, %1, %2, p;\n"
+      " selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "n"(kId), "n"(kThreads), "r"(ok ? 1 : 0)
+      : "memory");
+  return r != 0;
+}
+
+// Four floats at a shared-memory offset of another CTA of the cluster.
+__device__ __forceinline__ float4 ld_dsmem_v4f(uint32_t local_addr, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(map_shared_rank(local_addr, rank))
+               : "memory");
+  return v;
+}
+
+// Output element types by their zcutlass_dtype value.
+enum : int { kF16 = 0, kBf16 = 1, kF32 = 2 };
+
+__device__ __forceinline__ float load_out(const void* p, int64_t i, int type) {
+  if (type == kF32) return static_cast<const float*>(p)[i];
+  if (type == kBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const half*>(p)[i]);
+}
+__device__ __forceinline__ void store_out(void* p, int64_t i, int type, float v) {
+  if (type == kF32) static_cast<float*>(p)[i] = v;
+  else if (type == kBf16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<half*>(p)[i] = __float2half_rn(v);
+}
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi, int type) {
+  return type == kBf16 ? Elem<__nv_bfloat16>::pack(lo, hi) : Elem<half>::pack(lo, hi);
+}
+
+}  // namespace fp8
+}  // namespace zcb

@@ -3,12 +3,18 @@
 #include "layer_ops.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
+#include <cstdlib>
+#include <cstring>
 
 #include "kernels/fp8_generic_gemm.cuh"
 #include "kernels/quantize_fp8.cuh"
 #include "kernels/rotary.cuh"
+#include "kernels/sm100_fp8_pair.cuh"
+#include "kernels/sm100_fp8_swapab.cuh"
 #include "launchers.hpp"
+#include "tma_desc.hpp"
 
 namespace zcb {
 namespace {
@@ -64,6 +70,146 @@ cudaError_t generic_fp8(const Fp8GemmParams& p, bool a5, bool b5, cudaStream_t s
   auto go = [&](auto kernel) { return launch(kernel, tiles, kThreads, stream, p); };
   if (a5) return b5 ? go(gemm_kernel<Out, true, true>) : go(gemm_kernel<Out, true, false>);
   return b5 ? go(gemm_kernel<Out, false, true>) : go(gemm_kernel<Out, false, false>);
+}
+
+// ---------------------------------------------------------------- 8-bit product on tcgen05
+
+// One launch of a kernel with dynamic shared memory (its limit is raised once per device) in clusters of
+// `cluster` CTAs.
+template <typename... P, typename... A>
+cudaError_t launch_cluster(void (*kernel)(P...), std::atomic<uint64_t>& ready, const DeviceInfo& dev, int smem, int64_t grid,
+                           int threads, int cluster, cudaStream_t stream, const A&... args) {
+  if (grid < 1 || grid > INT_MAX) return cudaErrorInvalidValue;
+  const uint64_t bit = uint64_t(1) << (dev.ordinal & 63);
+  if ((ready.load(std::memory_order_acquire) & bit) == 0) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (programmatic_launch()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  count_launches(1);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+bool fp8_map(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t k, int64_t ld, int box_rows) {
+  return make_tma_2d(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, k, ld, box_rows, fp8::kBlockK, TmaSwizzle::B128);
+}
+
+struct Fp8Types {
+  bool a5, b5;
+  int d;  // zcutlass_dtype
+  int d_bytes() const { return d == ZCUTLASS_F32 ? 4 : 2; }
+};
+
+template <int MP, int STAGES, int KSUB>
+cudaError_t swap_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, int splits, cudaStream_t stream) {
+  using L = fp8_swap::Smem<MP, STAGES, KSUB>;
+  CUtensorMap tw, tx;
+  if (!fp8_map(&tw, g.b, g.n, g.k, g.ldb, fp8_swap::kBlockN) || !fp8_map(&tx, g.a, g.m, g.k, g.lda, MP))
+    return cudaErrorInvalidValue;
+  const int64_t tiles_m = div_up(g.m, MP);
+  Fp8SwapParams p{};
+  p.m = static_cast<int>(g.m), p.n = static_cast<int>(g.n);
+  p.num_kb = static_cast<int>(div_up(g.k, fp8::kBlockK));
+  p.splits = splits;
+  p.tiles_m = static_cast<int>(tiles_m);
+  p.a_scale = g.a_scale, p.a_scale_row = g.a_scale_row, p.a_scale_blk = g.a_scale_blk;
+  p.b_scale = g.b_scale, p.b_scale_row = g.b_scale_row, p.b_scale_blk = g.b_scale_blk;
+  p.d = g.d, p.ldd = g.ldd, p.d_type = t.d;
+  p.vec_d = g.ldd % 4 == 0 && aligned(g.d, 4 * t.d_bytes());
+  p.bias = g.bias;
+  p.idesc = fp8::idesc(fp8_swap::kBlockN, MP, t.b5, t.a5);
+  p.error_word = dev.error_word;
+  const int64_t grid = tiles_m * div_up(g.n, fp8_swap::kBlockN) * splits;
+  static std::atomic<uint64_t> ready[2];
+  if (g.b_scale_rows == 1)
+    return launch_cluster(fp8_swap::gemm_kernel<MP, STAGES, KSUB, true>, ready[1], dev, L::kDynamicBytes, grid,
+                          fp8_swap::kThreads, splits, stream, tw, tx, p);
+  return launch_cluster(fp8_swap::gemm_kernel<MP, STAGES, KSUB, false>, ready[0], dev, L::kDynamicBytes, grid,
+                        fp8_swap::kThreads, splits, stream, tw, tx, p);
+}
+
+cudaError_t pair_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, cudaStream_t stream) {
+  using L = fp8_pair::Smem;
+  CUtensorMap ta, tb, td{};
+  if (!fp8_map(&ta, g.a, g.m, g.k, g.lda, fp8_pair::kHalf) || !fp8_map(&tb, g.b, g.n, g.k, g.ldb, fp8_pair::kHalf))
+    return cudaErrorInvalidValue;
+  Fp8PairParams p{};
+  p.m = static_cast<int>(g.m), p.n = static_cast<int>(g.n);
+  p.num_kb = static_cast<int>(div_up(g.k, fp8::kBlockK));
+  p.tiles_m = static_cast<int>(div_up(g.m, fp8_pair::kBlock)), p.tiles_n = static_cast<int>(div_up(g.n, fp8_pair::kBlock));
+  if (static_cast<int64_t>(p.tiles_m) * p.tiles_n > INT_MAX - 1024) return cudaErrorInvalidValue;
+  p.total_tiles = p.tiles_m * p.tiles_n;
+  p.group_m = std::min(p.tiles_m, 8);
+  p.a_scale = g.a_scale, p.a_scale_row = g.a_scale_row, p.a_scale_blk = g.a_scale_blk;
+  p.b_scale = g.b_scale, p.b_scale_row = g.b_scale_row, p.b_scale_blk = g.b_scale_blk;
+  p.d = g.d, p.ldd = g.ldd, p.d_type = t.d;
+  const CUtensorMapDataType type = t.d == ZCUTLASS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : t.d == ZCUTLASS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  p.tma_d = aligned(g.d, 16) && g.ldd * t.d_bytes() % 16 == 0 &&
+            make_tma_2d(&td, g.d, type, t.d_bytes(), g.m, g.n, g.ldd, 32, 64 / t.d_bytes(), TmaSwizzle::B64);
+  p.bias = g.bias;
+  p.idesc = fp8::idesc(fp8_pair::kBlock, fp8_pair::kBlock, t.a5, t.b5);
+  p.error_word = dev.error_word;
+  const int64_t grid = 2 * std::min<int64_t>(p.total_tiles, dev.sm_count / 2);
+  static std::atomic<uint64_t> ready[2];
+  if (g.b_scale_rows == 1)
+    return launch_cluster(fp8_pair::gemm_kernel<true>, ready[1], dev, L::kDynamicBytes, grid, fp8_pair::kThreads, 2, stream,
+                          ta, tb, td, p);
+  return launch_cluster(fp8_pair::gemm_kernel<false>, ready[0], dev, L::kDynamicBytes, grid, fp8_pair::kThreads, 2, stream,
+                        ta, tb, td, p);
+}
+
+// ZCUTLASS_FORCE_KERNEL=fp8_generic | fp8_swap<rows> | fp8_pair pins the kernel of the 8-bit product
+// (tests); other values concern the 16-bit GEMM alone.
+bool forced(const char* kernel) {
+  const char* f = std::getenv("ZCUTLASS_FORCE_KERNEL");
+  return f != nullptr && std::strcmp(f, kernel) == 0;
+}
+bool any_forced() {
+  const char* f = std::getenv("ZCUTLASS_FORCE_KERNEL");
+  return f != nullptr && std::strncmp(f, "fp8_", 4) == 0;
+}
+
+// CTAs along K per tile of the swapped kernel: as many as fit the SMs' slots at once, each with at least
+// two blocks, at most a cluster of 8.
+int swap_splits(int64_t tiles, int64_t num_kb, int64_t slots) {
+  const char* v = std::getenv("ZCUTLASS_SPLITK");
+  int64_t s = v != nullptr && v[0] != '\0' ? std::atoi(v) : slots / std::max<int64_t>(tiles, 1);
+  s = std::min<int64_t>(s, std::min<int64_t>(fp8_swap::kMaxSplits, num_kb / 2));
+  return static_cast<int>(std::max<int64_t>(s, 1));
+}
+
+cudaError_t tensor_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, cudaStream_t stream) {
+  const int64_t tiles_n = div_up(g.n, 128), kb = div_up(g.k, fp8::kBlockK), sms = dev.sm_count;
+  const bool any = any_forced();
+  if (any ? forced("fp8_pair") : div_up(g.m, 256) * div_up(g.n, 256) >= sms / 4) return pair_fp8(g, t, dev, stream);
+  if (any ? forced("fp8_swap16") : g.m <= 16) return swap_fp8<16, 3, 2>(g, t, dev, swap_splits(tiles_n * div_up(g.m, 16), kb, 2 * sms), stream);
+  if (any ? forced("fp8_swap32") : g.m <= 32) return swap_fp8<32, 5, 1>(g, t, dev, swap_splits(tiles_n * div_up(g.m, 32), kb, 2 * sms), stream);
+  if (any ? forced("fp8_swap64") : g.m <= 64) return swap_fp8<64, 4, 1>(g, t, dev, swap_splits(tiles_n * div_up(g.m, 64), kb, 2 * sms), stream);
+  return swap_fp8<128, 3, 2>(g, t, dev, swap_splits(tiles_n * div_up(g.m, 128), kb, sms), stream);
 }
 
 template <typename T, int V>
@@ -136,6 +282,8 @@ cudaError_t launch_gemm_fp8(const zcutlass_fp8_gemm_desc& d, const void* a, cons
                         d.b_scale_rows, d.bias, info->error_word};
   const bool a5 = d.a_type == ZCUTLASS_E5M2, b5 = d.b_type == ZCUTLASS_E5M2;
   const cudaStream_t stream = static_cast<cudaStream_t>(d.stream);
+  if (d.k > 0 && aligned(a, 16) && aligned(b, 16) && d.lda % 16 == 0 && d.ldb % 16 == 0 && !forced("fp8_generic"))
+    return tensor_fp8(p, {a5, b5, d.d_type}, *info, stream);
   if (d.d_type == ZCUTLASS_F16) return generic_fp8<half>(p, a5, b5, stream);
   if (d.d_type == ZCUTLASS_BF16) return generic_fp8<__nv_bfloat16>(p, a5, b5, stream);
   return generic_fp8<float>(p, a5, b5, stream);

@@ -31,19 +31,24 @@ EncodeTiledFn encode_fn() {
 
 bool make_tma_2d(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols,
                  int64_t ld, int box_rows, int box_cols, TmaSwizzle swizzle) {
+  return make_tma_2d(map, base, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, rows,
+                     cols, ld, box_rows, box_cols, swizzle);
+}
+
+bool make_tma_2d(CUtensorMap* map, const void* base, CUtensorMapDataType type, int elem_bytes, int64_t rows,
+                 int64_t cols, int64_t ld, int box_rows, int box_cols, TmaSwizzle swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr || rows <= 0 || cols <= 0) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * static_cast<cuuint64_t>(elem_bytes)};
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t elem_strides[2] = {1, 1};
   const CUtensorMapSwizzle sw = swizzle == TmaSwizzle::B128  ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : swizzle == TmaSwizzle::B64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                              : CU_TENSOR_MAP_SWIZZLE_NONE;
-  const CUresult r =
-      fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-         const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, elem_strides,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }
 

@@ -18,6 +18,10 @@ enum class TmaSwizzle { None, B64, B128 };
 bool make_tma_2d(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols,
                  int64_t ld, int box_rows, int box_cols, TmaSwizzle swizzle);
 
+// The same for elements of any type of `elem_bytes` bytes.
+bool make_tma_2d(CUtensorMap* map, const void* base, CUtensorMapDataType type, int elem_bytes, int64_t rows,
+                 int64_t cols, int64_t ld, int box_rows, int box_cols, TmaSwizzle swizzle);
+
 // True when a matrix can be described by a TMA map: 16-byte aligned base and
 // a leading dimension whose byte size is a multiple of 16.
 inline bool tma_compatible(const void* base, int64_t ld_elems) {
