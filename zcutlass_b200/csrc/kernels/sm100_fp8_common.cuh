@@ -68,6 +68,30 @@ __device__ __forceinline__ void tmem_ld_wait_x16(uint32_t (&r)[16]) {
                : "memory");
 }
 
+// mbar_wait for waits that come once per k block: the timer that bounds it is first read after 64 tries,
+// since the read itself takes longer than such a wait.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const WaitCtx& ctx, int code) {
+  const uint32_t addr = smem_addr(bar);
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(addr, parity)) return true;
+  return mbar_wait(bar, parity, ctx, code);
+}
+
+// True in one lane of the (converged) warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+  return r != 0;
+}
+
+// Arrive on an mbarrier in another CTA of the cluster to say that a TMEM buffer has been read. No memory
+// contents are handed over (tcgen05.fence orders the TMEM reads), so the release is CTA-wide: at cluster
+// scope it waits for every load in flight, the scales fetched ahead among them (4x slower per block).
+__device__ __forceinline__ void arrive_read(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // Two 32-bit values in one register pair.
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
   uint64_t v;

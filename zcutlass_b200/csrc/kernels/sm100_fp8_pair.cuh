@@ -7,21 +7,33 @@
 // of two 256-column TMEM buffers; each CTA holds its 128 rows x 256 columns.
 // Eight accumulation warps per CTA (two per TMEM quarter, 128 columns each)
 // read the buffer and add it, scaled, into 128 32-bit accumulators per thread,
-// while the MMAs of the next block fill the other buffer. At full rate a block
-// takes the tensor pipe 512 cycles per SM, and the accumulation warps 128
-// columns x 8 warps: 256 cycles of TMEM reads and 128 of packed fma issue.
-// 128 accumulators, one TMEM chunk in use and one in flight need more than the
-// 168 registers three warps per SM sub-partition get: the first warpgroup hands
-// registers over (128 x 72 + 256 x 216 = 384 x 168).
+// while the MMAs of the next block fill the other buffer.
 //
-// With 128 x 128 weight scales the factor is one product per thread and block;
-// with a scale per row of B (kRows) the 128 column scales of a warpgroup go
-// through shared memory, two slots in turn.
+// What bounds it: at full rate a block takes the tensor pipe 512 cycles (531
+// measured), TMEM reads and 32-bit fma 260-350. A buffer's turnaround (MMAs,
+// commit, read, arrival at the leader) must fit two blocks' time, so nothing
+// slow may sit on it:
+//  - the warp that issues MMAs walks its loop as a whole, with its state in
+//    uniform registers and one lane issuing (per-lane descriptors alone halved
+//    the MMA rate: the accumulation warps leave few issue slots);
+//  - scales never pass through the accumulation warps' registers as loads in
+//    flight (a wait loop holds them up until the load returns): two otherwise
+//    idle warps, one per TMEM buffer, put each block's scales in shared memory
+//    and complete the buffer's `tmem_full` barrier together with the commit;
+//  - the arrival at the leader's `tmem_empty` is not a cluster-wide release.
 //
-// Roles per CTA: warp 0 TMA producer (stages of two k blocks: 2 x 32 KiB), warp
-// 1 TMEM allocation and, in the leader, MMA issue; warps 4-11 accumulate, then
-// write the tile (registers -> swizzled shared memory -> TMA, or row by row
-// where D is ragged or unaligned) while the next tile's first blocks run.
+// With 128 x 128 weight scales the factor is one product per thread and block.
+// With a scale per row of B (kRows) TMEM is read as 16 x 8 fragments, in which
+// a thread meets only 32 of the 128 columns: a quarter of the shared-memory
+// reads that a row per thread would need.
+//
+// Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocation and, in the
+// leader, MMA issue, warps 2-3 scales; warps 4-11 accumulate, then write the
+// tile (registers -> swizzled shared memory -> TMA, or row by row where D is
+// ragged or unaligned) while the next tile's first blocks run. 128 accumulators
+// and the TMEM chunks need more than the 168 registers three warps per SM
+// sub-partition get: the first warpgroup hands registers over
+// (128 x 72 + 256 x 216 = 384 x 168).
 #pragma once
 
 #include "sm100_fp8_common.cuh"
@@ -52,23 +64,23 @@ constexpr int kBlock = 256;   // tile edge
 constexpr int kThreads = 384;
 constexpr int kAuxThreads = 128;
 constexpr int kAccWarps = 8;
-constexpr int kStages = 3;
-constexpr int kSub = 2;       // k blocks per stage
 constexpr int kBufs = 2;
-constexpr int kAhead = 4;
+constexpr int kSlots = 4;     // blocks whose scales are in shared memory
 constexpr uint32_t kTmemCols = 512;
 
+template <bool kRows>
 struct Smem {
+  static constexpr int kStages = kRows ? 4 : 5;
   static constexpr int kOperand = kHalf * kBlockK;  // 16 KiB
-  static constexpr int kSubBytes = 2 * kOperand;
-  static constexpr int kStageBytes = kSub * kSubBytes;
+  static constexpr int kStageBytes = 2 * kOperand;
   static constexpr int kOutOff = kStages * kStageBytes;
-  static constexpr int kOutWarp = 4096;  // per accumulation warp
-  static constexpr int kScaleOff = kOutOff + kAccWarps * kOutWarp;  // [2 column halves][2 slots][128] floats
-  static constexpr int kBarOff = kScaleOff + 2 * 2 * kHalf * 4;
+  static constexpr int kOutWarp = 8192;  // per accumulation warp: four chunks of 32 rows x 64 bytes
+  static constexpr int kSlotFloats = kHalf + (kRows ? kBlock : 8);  // row scales, column (block) scales
+  static constexpr int kScaleOff = kOutOff + kAccWarps * kOutWarp;
+  static constexpr int kBarOff = kScaleOff + kSlots * kSlotFloats * 4;
   static constexpr int kNumBars = 2 * kStages + 2 * kBufs + 1;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
-  static constexpr int kDynamicBytes = kMiscOff + 16 + 1024 - 128;  // room to align a 128-byte aligned base to 1024
+  static constexpr int kDynamicBytes = kMiscOff + 8;
   static_assert(kDynamicBytes <= 232448, "shared memory budget exceeded");
 };
 
@@ -77,6 +89,8 @@ enum : int {
   kErrMmaFull = (34 << 4) | 2,
   kErrMmaTmemEmpty = (34 << 4) | 3,
   kErrAccTmemFull = (34 << 4) | 4,
+  kErrScaleTmemFull = (34 << 4) | 5,
+  kErrAlignment = (34 << 4) | 6,
 };
 
 // Tiles in groups of group_m tile rows, column by column, so that concurrent tiles share operands in L2.
@@ -90,13 +104,24 @@ __device__ __forceinline__ void raster(int tile, const Fp8PairParams& p, int& tm
   tn = in / rows;
 }
 
+// 16 rows x 8 columns of 32 bits per 4 registers: registers 4 g, 4 g + 1 hold columns 8 g + (lane % 4) * 2
+// and the next of row lane / 4, registers 4 g + 2, 4 g + 3 the same of row lane / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
 template <bool kRows>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                 const __grid_constant__ CUtensorMap tmap_d, const Fp8PairParams p) {
-  using L = Smem;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  using L = Smem<kRows>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);  // used in the leader
   uint64_t* empty = full + kStages;
   uint64_t* tmem_full = empty + kStages;
@@ -104,8 +129,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = tmem_empty + kBufs;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
+  float* const slots = reinterpret_cast<float*>(smem + L::kScaleOff);
 
-  const int warp = threadIdx.x >> 5;
+  if ((smem_addr(smem) & 1023u) != 0) {  // the swizzled tiles need it; every CTA has the same base
+    if (threadIdx.x == 0 && p.error_word != nullptr) atomicCAS(p.error_word, 0, kErrAlignment);
+    return;
+  }
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
@@ -116,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < kBufs; ++b) {
-      mbar_init(&tmem_full[b], 1);
+      mbar_init(&tmem_full[b], 2);  // the commit and the scales
       mbar_init(&tmem_empty[b], 2 * kAccWarps);
     }
     mbar_init(drain, 1);
@@ -155,22 +185,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           raster(tile, p, tm, tn);
           const int m0 = tm * kBlock + static_cast<int>(rank) * kHalf;
           const int n0 = tn * kBlock + static_cast<int>(rank) * kHalf;
-          for (int kb = 0; kb < p.num_kb; kb += kSub, ++it) {
+          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
             const uint32_t s = it % kStages;
-            if (!mbar_wait(&empty[s], ((it / kStages) & 1u) ^ 1u, ctx, kErrProducerEmpty)) {
+            if (!fp8::wait(&empty[s], ((it / kStages) & 1u) ^ 1u, ctx, kErrProducerEmpty)) {
               ok = false;
               break;
             }
-            const int subs = p.num_kb - kb < kSub ? p.num_kb - kb : kSub;
             const uint32_t full_leader = map_shared_rank(smem_addr(&full[s]), 0);
-            if (leader) mbar_arrive_expect_tx(&full[s], 2 * subs * L::kSubBytes);
-  #pragma unroll
-            for (int sub = 0; sub < kSub; ++sub) {
-              if (sub >= subs) break;
-              uint8_t* at = smem + s * L::kStageBytes + sub * L::kSubBytes;
-              tma_load_2d_pair(at, &tmap_a, full_leader, (kb + sub) * kBlockK, m0);
-              tma_load_2d_pair(at + L::kOperand, &tmap_b, full_leader, (kb + sub) * kBlockK, n0);
-            }
+            if (leader) mbar_arrive_expect_tx(&full[s], 2 * L::kStageBytes);
+            uint8_t* at = smem + s * L::kStageBytes;
+            tma_load_2d_pair(at, &tmap_a, full_leader, kb * kBlockK, m0);
+            tma_load_2d_pair(at + L::kOperand, &tmap_b, full_leader, kb * kBlockK, n0);
           }
         }
         if (!ok) {  // unwind: loads already issued must land before the CTAs can exit
@@ -185,168 +210,218 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer (leader only)
-      if (leader && lane == 0) {
-        uint32_t it = 0, i = 0;  // stages and k blocks so far
+      if (leader) {
+        const bool one = fp8::elect_one();
+        uint32_t s = 0, phase = 0, buf = 0, buf_phase = 1;
         bool ok = true, issued = false;
+        const uint64_t desc0 = smem_desc_sw128(smem_addr(smem), 16, 1024);
         for (int tile = pair; ok && tile < p.total_tiles; tile += npairs) {
-          for (int kb = 0; ok && kb < p.num_kb; kb += kSub, ++it) {
-            const uint32_t s = it % kStages;
-            if (!mbar_wait(&full[s], (it / kStages) & 1u, ctx, kErrMmaFull)) {
-              ok = false;
-              break;
-            }
-            const int subs = p.num_kb - kb < kSub ? p.num_kb - kb : kSub;
-            for (int sub = 0; sub < subs; ++sub, ++i) {
-              const uint32_t buf = i % kBufs;
-              if (!mbar_wait(&tmem_empty[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrMmaTmemEmpty)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after_sync();
-              const uint32_t a = smem_addr(smem + s * L::kStageBytes + sub * L::kSubBytes);
-  #pragma unroll
+          for (int kb = 0; kb < p.num_kb; ++kb) {
+            ok = fp8::wait(&full[s], phase, ctx, kErrMmaFull);
+            ok = ok && fp8::wait(&tmem_empty[buf], buf_phase, ctx, kErrMmaTmemEmpty);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after_sync();
+            if (one) {
+              const uint64_t a = desc0 + (s * L::kStageBytes >> 4);
+#pragma unroll
               for (int kk = 0; kk < kBlockK / fp8::kMmaK; ++kk)
-                fp8::mma_pair(tmem_base + buf * kBlock, smem_desc_sw128(a + kk * fp8::kMmaK, 16, 1024),
-                              smem_desc_sw128(a + L::kOperand + kk * fp8::kMmaK, 16, 1024), p.idesc, kk != 0 ? 1u : 0u);
-              issued = true;
+                fp8::mma_pair(tmem_base + buf * kBlock, a + (kk * fp8::kMmaK >> 4),
+                              a + ((L::kOperand + kk * fp8::kMmaK) >> 4), p.idesc, kk != 0 ? 1u : 0u);
               umma_commit_pair_multicast(&tmem_full[buf], 0x3);
+              umma_commit_pair_multicast(&empty[s], 0x3);
             }
-            if (ok) umma_commit_pair_multicast(&empty[s], 0x3);
+            __syncwarp();
+            issued = true;
+            buf ^= 1u;
+            buf_phase ^= buf == 0 ? 1u : 0u;
+            if (++s == kStages) s = 0, phase ^= 1u;
           }
         }
-        if (!ok && issued) {
+        if (!ok && issued && one) {
           umma_commit_pair_multicast(drain, 0x1);
           mbar_wait_quiet(drain, 0, 200000000ull);
         }
       }
       __syncwarp();
+    } else {
+      // ------------------------------------------------------------ scales (both CTAs)
+      // Warp 2 + b serves the blocks of TMEM buffer b. Slot i % 4 is rewritten once phase i - 2 of the buffer
+      // is complete: its MMAs were issued after every warp had read block i - 4.
+      const uint32_t buf = static_cast<uint32_t>(warp - 2);
+      uint32_t i = 0;  // blocks so far, both buffers'
+      bool ok = true;
+      for (int tile = pair; ok && tile < p.total_tiles; tile += npairs) {
+        int tm, tn;
+        raster(tile, p, tm, tn);
+        const int64_t m0 = static_cast<int64_t>(tm) * kBlock + rank * kHalf;
+        const int64_t n0 = static_cast<int64_t>(tn) * kBlock;
+        for (int kb = 0; ok && kb < p.num_kb; ++kb, ++i) {
+          if ((i & 1u) != buf) continue;
+          const float* sa = p.a_scale + kb * p.a_scale_blk;
+          const float* sb = p.b_scale + kb * p.b_scale_blk;
+          float a[kHalf / 32], b[kRows ? kBlock / 32 : 1];
+#pragma unroll
+          for (int j = 0; j < kHalf / 32; ++j) {
+            const int64_t row = m0 + j * 32 + lane;
+            a[j] = row < p.m ? __ldg(sa + row * p.a_scale_row) : 0.0f;
+          }
+          if constexpr (kRows) {
+#pragma unroll
+            for (int j = 0; j < kBlock / 32; ++j) {
+              const int64_t col = n0 + j * 32 + lane;
+              b[j] = col < p.n ? __ldg(sb + col * p.b_scale_row) : 0.0f;
+            }
+          } else {
+            b[0] = lane < 2 && n0 + lane * kHalf < p.n ? __ldg(sb + (n0 / kHalf + lane) * p.b_scale_row) : 0.0f;
+          }
+          if (i >= kBufs) ok = fp8::wait(&tmem_full[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrScaleTmemFull);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          float* slot = slots + (i % kSlots) * L::kSlotFloats;
+#pragma unroll
+          for (int j = 0; j < kHalf / 32; ++j) slot[j * 32 + lane] = a[j];
+          if constexpr (kRows) {
+#pragma unroll
+            for (int j = 0; j < kBlock / 32; ++j) slot[kHalf + j * 32 + lane] = b[j];
+          } else {
+            if (lane < 2) slot[kHalf + lane] = b[0];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tmem_full[buf]);
+        }
+      }
     }
   } else {
     // ------------------------------------------------------------ accumulation and output (both CTAs)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int quarter = warp & 3;
     const int w = warp - kAuxThreads / 32;
-    const int half = w >> 2;                              // columns half * 128 ..
-    const int t = threadIdx.x & (kHalf - 1);              // thread of the half's warpgroup
-    float* scales = reinterpret_cast<float*>(smem + L::kScaleOff) + half * 2 * kHalf;
+    const int half = w >> 2;  // columns half * 128 ..
     uint8_t* out = smem + L::kOutOff + w * L::kOutWarp;
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * kHalf;
     uint32_t i = 0;
     uint32_t chunk = 0;
     bool ok = true;
-    const float* sa = nullptr;
-    const float* sb = nullptr;
-    bool row_ok = false, col_ok = false;
-    float a_next[kAhead], b_next[kAhead];
-    auto fetch = [&](int kb, float& a, float& b) {
-      const bool in = kb < p.num_kb;
-      a = in && row_ok ? __ldg(sa + kb * p.a_scale_blk) : 0.0f;
-      b = in && col_ok ? __ldg(sb + kb * p.b_scale_blk) : 0.0f;
-    };
-    auto start = [&](int tile) {  // the first scales of a tile
-      if (tile >= p.total_tiles) return;
-      int tm, tn;
-      raster(tile, p, tm, tn);
-      const int64_t row = static_cast<int64_t>(tm) * kBlock + rank * kHalf + quarter * 32 + lane;
-      const int64_t n0 = static_cast<int64_t>(tn) * kBlock + half * kHalf;
-      const int64_t b = kRows ? n0 + t : n0 / kHalf;
-      row_ok = row < p.m;
-      col_ok = kRows ? n0 + t < p.n : n0 < p.n;
-      sa = p.a_scale + row * p.a_scale_row;
-      sb = p.b_scale + b * p.b_scale_row;
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) fetch(u, a_next[u], b_next[u]);
-    };
-    start(pair);
     for (int tile = pair; ok && tile < p.total_tiles; tile += npairs) {
       int tm, tn;
       raster(tile, p, tm, tn);
       const int m0 = tm * kBlock + static_cast<int>(rank) * kHalf + quarter * 32;  // the warp's first row
       const int n0 = tn * kBlock + half * kHalf;
-      uint64_t acc[kHalf / 2];
+      // One row per thread: values 0..127 are its columns. kRows: values 32 c + 16 h + 4 g + e are fragment
+      // element e of column group 4 c + g of the 16 rows h.
+      float acc[kHalf];
 #pragma unroll
-      for (int j = 0; j < kHalf / 2; ++j) acc[j] = 0;
+      for (int j = 0; j < kHalf; ++j) acc[j] = 0.0f;
 #pragma unroll 1
-      for (int kb = 0; kb < p.num_kb; ++kb) {
+      for (int kb = 0; kb < p.num_kb; ++kb, ++i) {
         const uint32_t buf = i % kBufs;
-        float* slot = scales + (i & 1u) * kHalf;  // blocks of successive tiles keep alternating
-        const uint64_t mine = fp8::both(kRows ? a_next[0] : a_next[0] * b_next[0]);
-        if constexpr (kRows) slot[t] = b_next[0];
-#pragma unroll
-        for (int u = 0; u + 1 < kAhead; ++u) a_next[u] = a_next[u + 1], b_next[u] = b_next[u + 1];
-        fetch(kb + kAhead, a_next[kAhead - 1], b_next[kAhead - 1]);
-        ok = mbar_wait(&tmem_full[buf], (i / kBufs) & 1u, ctx, kErrAccTmemFull);
-        if constexpr (kRows) ok = half == 0 ? fp8::barrier_and<1, kHalf>(ok) : fp8::barrier_and<2, kHalf>(ok);
-        else ok = __all_sync(0xffffffffu, ok);
+        const float* slot = slots + (i % kSlots) * L::kSlotFloats;
+        ok = fp8::wait(&tmem_full[buf], (i / kBufs) & 1u, ctx, kErrAccTmemFull);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        ++i;
         tc_fence_after_sync();
         uint32_t v[2][16];
-        fp8::tmem_ld_x16(taddr + buf * kBlock, v[0]);
+        const uint32_t t0 = taddr + buf * kBlock;
+        if constexpr (!kRows) {
+          fp8::tmem_ld_x16(t0, v[0]);
+          const float scale = slot[quarter * 32 + lane] * slot[kHalf + half];
 #pragma unroll
-        for (int c = 0; c < kHalf / 16; ++c) {
-          uint32_t(&r)[16] = v[c & 1];
-          fp8::tmem_ld_wait_x16(r);
-          if (c + 1 < kHalf / 16) {
-            fp8::tmem_ld_x16(taddr + buf * kBlock + (c + 1) * 16, v[(c + 1) & 1]);
-          } else {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
-          }
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            uint64_t s0 = mine, s1 = mine;
-            if constexpr (kRows) {
-              const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(slot + c * 16 + j);
-              s0 = fp8::mul2(s.x, mine);
-              s1 = fp8::mul2(s.y, mine);
+          for (int c = 0; c < kHalf / 16; ++c) {
+            uint32_t(&r)[16] = v[c & 1];
+            fp8::tmem_ld_wait_x16(r);
+            if (c + 1 < kHalf / 16) {
+              fp8::tmem_ld_x16(t0 + (c + 1) * 16, v[(c + 1) & 1]);
+            } else {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
             }
-            fp8::fma2(acc[c * 8 + j / 2], s0, fp8::pack2(r[j], r[j + 1]));
-            fp8::fma2(acc[c * 8 + j / 2 + 1], s1, fp8::pack2(r[j + 2], r[j + 3]));
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(scale, __uint_as_float(r[j]), acc[c * 16 + j]);
+          }
+        } else {
+          tmem_ld_16x256b_x4(t0, v[0]);
+          float sa[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sa[j] = slot[quarter * 32 + j * 8 + (lane >> 2)];
+          const float2* sb = reinterpret_cast<const float2*>(slot + kHalf + half * kHalf) + (lane & 3);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {  // 32 columns of 16 rows per step: (c / 2, c % 2)
+            uint32_t(&r)[16] = v[c & 1];
+            fp8::tmem_ld_wait_x16(r);
+            if (c + 1 < 8) {
+              tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, v[(c + 1) & 1]);
+            } else {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
+            }
+            const float lo = sa[2 * (c & 1)], hi = sa[2 * (c & 1) + 1];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float2 s = sb[((c >> 1) * 4 + g) * 4];
+              float* q = acc + (c >> 1) * 32 + (c & 1) * 16 + 4 * g;
+              q[0] = fmaf(s.x * lo, __uint_as_float(r[4 * g]), q[0]);
+              q[1] = fmaf(s.y * lo, __uint_as_float(r[4 * g + 1]), q[1]);
+              q[2] = fmaf(s.x * hi, __uint_as_float(r[4 * g + 2]), q[2]);
+              q[3] = fmaf(s.y * hi, __uint_as_float(r[4 * g + 3]), q[3]);
+            }
           }
         }
       }
       if (!ok) break;
-      start(tile + npairs);  // on their way while this tile is written
+      // Chunks of 32 rows x 64 bytes (32 values of 16 bits, 16 of 32) go out by TMA, four in flight.
       const bool wide = p.d_type == fp8::kF32;
-      // Chunks of 64 bytes per row (32 values of 16 bits, 16 of 32) go out by TMA, double-buffered.
 #pragma unroll
       for (int c = 0; c < kHalf / 32; ++c) {
         const int nc = n0 + c * 32;
         if (nc >= p.n || m0 >= p.m) break;
-        float v[32];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float2 f = fp8::unpack2(acc[c * 16 + j]);
-          v[2 * j] = f.x;
-          v[2 * j + 1] = f.y;
-        }
+        float* v = acc + c * 32;
         if (p.bias != nullptr) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (nc + j < p.n) v[j] += fp8::load_out(p.bias, nc + j, p.d_type);
+          for (int j = 0; j < 32; ++j) {
+            const int col = kRows ? 8 * ((j >> 2) & 3) + 2 * (lane & 3) + (j & 1) : j;
+            if (nc + col < p.n) v[j] += fp8::load_out(p.bias, nc + col, p.d_type);
+          }
         }
         if (p.tma_d && nc + 32 <= p.n) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (h == 1 && !wide) break;
-            uint8_t* buf = out + (chunk & 1u) * 2048;
-            if (lane == 0) bulk_wait_group_read<1>();
+            uint8_t* buf = out + (chunk & 3u) * 2048;
+            if (lane == 0) bulk_wait_group_read<3>();
             __syncwarp();
-            uint4* row = reinterpret_cast<uint4*>(buf + lane * 64);
+            if constexpr (!kRows) {
+              uint4* row = reinterpret_cast<uint4*>(buf + lane * 64);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4 word;
-              if (wide) {
-                const float* f = v + h * 16 + 4 * q;
-                word = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-              } else {
-                const float* f = v + 8 * q;
-                word = make_uint4(fp8::pack_out(f[0], f[1], p.d_type), fp8::pack_out(f[2], f[3], p.d_type),
-                                  fp8::pack_out(f[4], f[5], p.d_type), fp8::pack_out(f[6], f[7], p.d_type));
+              for (int q = 0; q < 4; ++q) {
+                uint4 word;
+                if (wide) {
+                  const float* f = v + h * 16 + 4 * q;
+                  word = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+                } else {
+                  const float* f = v + 8 * q;
+                  word = make_uint4(fp8::pack_out(f[0], f[1], p.d_type), fp8::pack_out(f[2], f[3], p.d_type),
+                                    fp8::pack_out(f[4], f[5], p.d_type), fp8::pack_out(f[6], f[7], p.d_type));
+                }
+                row[q ^ ((lane >> 1) & 3)] = word;
               }
-              row[q ^ ((lane >> 1) & 3)] = word;
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {  // rows 16 (j / 16) + 8 (j % 4 / 2) + lane / 4, group j / 4 % 4
+                const int row = 16 * (j >> 4) + 8 * ((j >> 1) & 1) + (lane >> 2);
+                const int g = (j >> 2) & 3;
+                if (wide) {
+                  if ((g >> 1) != h) continue;
+                  const int unit = 2 * (g & 1) + ((lane & 3) >> 1);  // 16 bytes: 4 columns
+                  *reinterpret_cast<float2*>(buf + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4) + (lane & 1) * 8) =
+                      make_float2(v[j], v[j + 1]);
+                } else {
+                  *reinterpret_cast<uint32_t*>(buf + row * 64 + ((g ^ ((row >> 1) & 3)) << 4) + (lane & 3) * 4) =
+                      fp8::pack_out(v[j], v[j + 1], p.d_type);
+                }
+              }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -361,10 +436,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
           float* stage = reinterpret_cast<float*>(out);
+          if constexpr (!kRows) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4*>(stage + lane * 32 + 4 * (q ^ (lane & 7))) =
-                make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<float4*>(stage + lane * 32 + 4 * (q ^ (lane & 7))) =
+                  make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const int row = 16 * (j >> 4) + 8 * ((j >> 1) & 1) + (lane >> 2);
+              const int unit = 2 * ((j >> 2) & 3) + ((lane & 3) >> 1);
+              *reinterpret_cast<float2*>(stage + row * 32 + 4 * (unit ^ (row & 7)) + 2 * (lane & 1)) = make_float2(v[j], v[j + 1]);
+            }
+          }
           __syncwarp();
           const int rows = p.m - m0 < 32 ? p.m - m0 : 32;
           if (nc + lane < p.n) {

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, MP == 128 ? 1 : 2)
       bool ok = true;
       for (int kb = kb0; kb < kb1; kb += KSUB, ++it) {
         const uint32_t s = it % STAGES;
-        if (!mbar_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, ctx, kErrProducerEmpty)) {
+        if (!fp8::wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, ctx, kErrProducerEmpty)) {
           ok = false;
           break;
         }
@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(kThreads, MP == 128 ? 1 : 2)
       for (int kb = kb0; ok && kb < kb1; ++kb, ++i) {
         const uint32_t it = i / KSUB, sub = i % KSUB, s = it % STAGES;
         const uint32_t buf = i % kBufs;
-        if (!mbar_wait(&tmem_empty[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrMmaTmemEmpty) ||
-            (sub == 0 && !mbar_wait(&full[s], (it / STAGES) & 1u, ctx, kErrMmaFull))) {
+        if (!fp8::wait(&tmem_empty[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrMmaTmemEmpty) ||
+            (sub == 0 && !fp8::wait(&full[s], (it / STAGES) & 1u, ctx, kErrMmaFull))) {
           ok = false;
           break;
         }
@@ -202,43 +202,46 @@ __global__ void __launch_bounds__(kThreads, MP == 128 ? 1 : 2)
 #pragma unroll
     for (int j = 0; j < MP / 2; ++j) acc[j] = 0;
     bool ok = true;
+    // Unrolled by the distance of the scale loads: each has a register of its own until it is used.
 #pragma unroll 1
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const uint32_t i = static_cast<uint32_t>(kb - kb0);
-      const uint32_t buf = i % kBufs;
-      float* slot = scales + (i & 1u) * MP;
-      if (t < MP) slot[t] = kRows ? a_next[0] : a_next[0] * b_next[0];
-      const uint64_t mine = fp8::both(b_next[0]);
+    for (int kb = kb0; ok && kb < kb1; kb += kAhead) {
 #pragma unroll
-      for (int u = 0; u + 1 < kAhead; ++u) a_next[u] = a_next[u + 1], b_next[u] = b_next[u + 1];
-      fetch(kb + kAhead, a_next[kAhead - 1], b_next[kAhead - 1]);
-      ok = mbar_wait(&tmem_full[buf], (i / kBufs) & 1u, ctx, kErrAccTmemFull);
-      ok = fp8::barrier_and<1, kAccThreads>(ok);  // the slot is written; all four warps go on, or none
-      if (!ok) break;
-      tc_fence_after_sync();
-      uint32_t v[2][16];
-      fp8::tmem_ld_x16(taddr + buf * MP, v[0]);
+      for (int u = 0; u < kAhead; ++u) {
+        if (kb + u >= kb1) break;
+        const uint32_t i = static_cast<uint32_t>(kb + u - kb0);
+        const uint32_t buf = i % kBufs;
+        float* slot = scales + (i & 1u) * MP;
+        if (t < MP) slot[t] = kRows ? a_next[u] : a_next[u] * b_next[u];
+        const uint64_t mine = fp8::both(b_next[u]);
+        fetch(kb + u + kAhead, a_next[u], b_next[u]);
+        ok = fp8::wait(&tmem_full[buf], (i / kBufs) & 1u, ctx, kErrAccTmemFull);
+        ok = fp8::barrier_and<1, kAccThreads>(ok);  // the slot is written; all four warps go on, or none
+        if (!ok) break;
+        tc_fence_after_sync();
+        uint32_t v[2][16];
+        fp8::tmem_ld_x16(taddr + buf * MP, v[0]);
 #pragma unroll
-      for (int c = 0; c < MP / 16; ++c) {
-        uint32_t(&w)[16] = v[c & 1];
-        fp8::tmem_ld_wait_x16(w);
-        if (c + 1 < MP / 16) {
-          fp8::tmem_ld_x16(taddr + buf * MP + (c + 1) * 16, v[(c + 1) & 1]);
-        } else {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&tmem_empty[buf]);
-        }
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(slot + c * 16 + j);
-          uint64_t s0 = s.x, s1 = s.y;
-          if constexpr (kRows) {
-            s0 = fp8::mul2(s0, mine);
-            s1 = fp8::mul2(s1, mine);
+        for (int c = 0; c < MP / 16; ++c) {
+          uint32_t(&w)[16] = v[c & 1];
+          fp8::tmem_ld_wait_x16(w);
+          if (c + 1 < MP / 16) {
+            fp8::tmem_ld_x16(taddr + buf * MP + (c + 1) * 16, v[(c + 1) & 1]);
+          } else {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tmem_empty[buf]);
           }
-          fp8::fma2(acc[c * 8 + j / 2], s0, fp8::pack2(w[j], w[j + 1]));
-          fp8::fma2(acc[c * 8 + j / 2 + 1], s1, fp8::pack2(w[j + 2], w[j + 3]));
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(slot + c * 16 + j);
+            uint64_t s0 = s.x, s1 = s.y;
+            if constexpr (kRows) {
+              s0 = fp8::mul2(s0, mine);
+              s1 = fp8::mul2(s1, mine);
+            }
+            fp8::fma2(acc[c * 8 + j / 2], s0, fp8::pack2(w[j], w[j + 1]));
+            fp8::fma2(acc[c * 8 + j / 2 + 1], s1, fp8::pack2(w[j + 2], w[j + 3]));
+          }
         }
       }
     }

@@ -151,7 +151,6 @@ cudaError_t swap_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo
 }
 
 cudaError_t pair_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, cudaStream_t stream) {
-  using L = fp8_pair::Smem;
   CUtensorMap ta, tb, td{};
   if (!fp8_map(&ta, g.a, g.m, g.k, g.lda, fp8_pair::kHalf) || !fp8_map(&tb, g.b, g.n, g.k, g.ldb, fp8_pair::kHalf))
     return cudaErrorInvalidValue;
@@ -161,7 +160,7 @@ cudaError_t pair_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo
   p.tiles_m = static_cast<int>(div_up(g.m, fp8_pair::kBlock)), p.tiles_n = static_cast<int>(div_up(g.n, fp8_pair::kBlock));
   if (static_cast<int64_t>(p.tiles_m) * p.tiles_n > INT_MAX - 1024) return cudaErrorInvalidValue;
   p.total_tiles = p.tiles_m * p.tiles_n;
-  p.group_m = std::min(p.tiles_m, 8);
+  p.group_m = std::min(p.tiles_m, 16);
   p.a_scale = g.a_scale, p.a_scale_row = g.a_scale_row, p.a_scale_blk = g.a_scale_blk;
   p.b_scale = g.b_scale, p.b_scale_row = g.b_scale_row, p.b_scale_blk = g.b_scale_blk;
   p.d = g.d, p.ldd = g.ldd, p.d_type = t.d;
@@ -176,9 +175,11 @@ cudaError_t pair_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo
   const int64_t grid = 2 * std::min<int64_t>(p.total_tiles, dev.sm_count / 2);
   static std::atomic<uint64_t> ready[2];
   if (g.b_scale_rows == 1)
-    return launch_cluster(fp8_pair::gemm_kernel<true>, ready[1], dev, L::kDynamicBytes, grid, fp8_pair::kThreads, 2, stream,
+    return launch_cluster(fp8_pair::gemm_kernel<true>, ready[1], dev, fp8_pair::Smem<true>::kDynamicBytes, grid,
+                          fp8_pair::kThreads, 2, stream,
                           ta, tb, td, p);
-  return launch_cluster(fp8_pair::gemm_kernel<false>, ready[0], dev, L::kDynamicBytes, grid, fp8_pair::kThreads, 2, stream,
+  return launch_cluster(fp8_pair::gemm_kernel<false>, ready[0], dev, fp8_pair::Smem<false>::kDynamicBytes, grid,
+                        fp8_pair::kThreads, 2, stream,
                         ta, tb, td, p);
 }
 
