@@ -39,8 +39,6 @@ constexpr int kRowThreads = 256;
 constexpr int kLaneVals = 16;                          // values per lane in the row kernel
 constexpr int kWarpVals = 32 * kLaneVals;              // 512 columns (4 groups) of one row per warp
 constexpr int kTileThreads = 256;
-constexpr int kTileVals = 8;                           // the tile kernel's threads hold 8 x 8 values
-constexpr int kTilePitch = kGroup + 16;                // bytes per transposed row in shared memory
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
@@ -155,116 +153,236 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const QuantizeParams 
   }
 }
 
+// Eight values as they are loaded: 16-bit types stay packed, so that a thread's 64 values take 32 registers
+// and three blocks fit an SM (two, with the values unpacked, kept too few loads in flight).
+template <typename T>
+struct Raw8 {
+  static constexpr int kWords = 8 * sizeof(T) / 4;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* p, int64_t n, bool vec) {
+    if (n >= 8 && vec) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+        w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = i < n ? __float_as_uint(p[i]) : 0u;
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = (2 * i < n ? h[2 * i] : 0u) | (2 * i + 1 < n ? static_cast<uint32_t>(h[2 * i + 1]) << 16 : 0u);
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    else {
+      const float2 f = Elem<T>::unpack(w[j >> 1]);
+      return (j & 1) ? f.y : f.x;
+    }
+  }
+};
+
+// The largest magnitudes of words: 32-bit values, or the two 16-bit values of a word each on its own. Both are
+// ordered as their bits are, infinities and NaN on top.
+template <typename T>
+__device__ __forceinline__ uint32_t max_mag(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4) return max(a, b);
+  else return __vmaxu2(a, b);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t mag(uint32_t w) {
+  return w & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu);
+}
+// A magnitude as the bits of a 32-bit value (16-bit types: the low half).
+template <typename T>
+__device__ __forceinline__ uint32_t mag_bits(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return m;
+  else return __float_as_uint(Elem<T>::unpack(m).x);
+}
+
 // A 128 x 128 tile per block, read once: 16 threads cover a row (8 columns each) and hold 8 consecutive
 // rows, so a thread's 8 x 8 values give 8 bytes of a row and 8 bytes of a column of the results. The
-// transposed bytes go through shared memory to be written as whole 128-byte rows.
+// transposed bytes go through shared memory to be written as whole 128-byte rows; their 16-byte units are
+// permuted by the column's eighth, so that the 16 threads of a row (8 columns apart) meet different banks.
 // kBlock: one scale for the tile; else one per row (kRows) and one per column (kCols) of it.
 template <typename T, int kTop, bool kRows, bool kCols, bool kBlock>
-__global__ void __launch_bounds__(kTileThreads) tile_kernel(const QuantizeParams p, bool vec_in, bool vec_q, bool vec_qt) {
-  __shared__ uint32_t col_amax[16][kGroup];
-  __shared__ float col_part[16][kGroup];
-  __shared__ Scale col_scale[kGroup];
-  __shared__ __align__(16) uint8_t turned[kGroup * kTilePitch];
-  __shared__ uint32_t warp_amax[kTileThreads / 32];
+__global__ void __launch_bounds__(kTileThreads, sizeof(T) == 4 ? 2 : 3)
+    tile_kernel(const QuantizeParams p, bool vec_in, bool vec_q, bool vec_qt) {
+  constexpr int kWarps = kTileThreads / 32;
+  constexpr bool kColStats = kCols && !kBlock;
+  constexpr int kWords = Raw8<T>::kWords;
+  __shared__ __align__(16) uint32_t col_amax[kColStats ? kWarps : 1][kGroup * sizeof(T) / 4];
+  __shared__ __align__(16) float col_part[kColStats ? kWarps : 1][kGroup];
+  __shared__ __align__(16) float col_inverse[kGroup];
+  __shared__ __align__(16) uint8_t turned[kCols ? kGroup * kGroup : 16];
+  __shared__ uint32_t warp_amax[kWarps];
   griddep_wait();
   griddep_launch_dependents();
   const int slot = threadIdx.x >> 4;         // 8 rows
+  const int warp = threadIdx.x >> 5;
   const int c0 = (threadIdx.x & 15) * 8;     // 8 columns
   const int64_t tiles_c = (p.cols + kGroup - 1) / kGroup;
-  const int64_t tr = blockIdx.x / tiles_c, tc = blockIdx.x % tiles_c;
+  const int64_t tr = blockIdx.x / tiles_c, tc = blockIdx.x - tr * tiles_c;
   const int64_t row0 = tr * kGroup + slot * 8, col0 = tc * kGroup + c0;
   const int64_t n = p.cols - col0;
-  float v[8][8];
+  Raw8<T> v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    load8(static_cast<const T*>(p.x) + (row0 + i) * p.ldx + col0, row0 + i < p.rows ? n : 0, vec_in, v[i]);
+    v[i].load(static_cast<const T*>(p.x) + (row0 + i) * p.ldx + col0, row0 + i < p.rows ? n : 0, vec_in);
 
   Scale block_scale{1.0f, 1.0f};
   if constexpr (kBlock) {
-    uint32_t amax = 0;
+    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max(amax, abs_bits(v[i][j]));
+      for (int j = 0; j < kWords; ++j) m = max_mag<T>(m, mag<T>(v[i].w[j]));
+    uint32_t amax = mag_bits<T>(m);
+    if constexpr (sizeof(T) == 2) amax = max(amax, mag_bits<T>(m >> 16));
     amax = __reduce_max_sync(0xffffffffu, amax);
-    if ((threadIdx.x & 31) == 0) warp_amax[threadIdx.x >> 5] = amax;
+    if ((threadIdx.x & 31) == 0) warp_amax[warp] = amax;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kTileThreads / 32; ++w) amax = max(amax, warp_amax[w]);
+    for (int w = 0; w < kWarps; ++w) amax = max(amax, warp_amax[w]);
     block_scale = scale_of<kTop>(amax);
     if (threadIdx.x == 0) {
       if (kRows) p.scale[tr * p.scale_row + tc * p.scale_blk] = block_scale.s;
       if (kCols) p.scale_t[tc * p.scale_t_row + tr * p.scale_t_blk] = block_scale.s;
     }
   }
+  if constexpr (kColStats) {
+    // Column maxima over the thread's 8 rows, then over the warp's two slots.
+    uint32_t m[kWords] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) m[j] = max_mag<T>(m[j], mag<T>(v[i].w[j]));
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) m[j] = max_mag<T>(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+    if ((threadIdx.x & 16) == 0) {
+#pragma unroll
+      for (int j = 0; j < kWords; j += 4)
+        *reinterpret_cast<uint4*>(&col_amax[warp][(threadIdx.x & 15) * kWords + j]) = make_uint4(m[j], m[j + 1], m[j + 2], m[j + 3]);
+    }
+    if (p.col_sums != nullptr) {
+      float sum[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sum[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[j] += v[i].get(j);
+        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 16);
+      }
+      if ((threadIdx.x & 16) == 0) {
+        *reinterpret_cast<float4*>(&col_part[warp][c0]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        *reinterpret_cast<float4*>(&col_part[warp][c0 + 4]) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < kGroup) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        uint32_t word = col_amax[w][threadIdx.x * sizeof(T) / 4];
+        if constexpr (sizeof(T) == 2) word = (threadIdx.x & 1) ? word >> 16 : word & 0xffffu;
+        amax = max(amax, word);
+      }
+      const Scale s = scale_of<kTop>(mag_bits<T>(amax));
+      col_inverse[threadIdx.x] = s.inverse;
+      const int64_t c = tc * kGroup + threadIdx.x;
+      if (c < p.cols) {
+        p.scale_t[c * p.scale_t_row + tr * p.scale_t_blk] = s.s;
+        if (p.col_sums != nullptr) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) sum += col_part[w][threadIdx.x];
+          p.col_sums[tr * p.cols + c] = sum;
+        }
+      }
+    }
+    __syncthreads();
+  }
   if constexpr (kRows) {
+    // Row maxima over 16 threads. Each exchange halves the rows a thread is responsible for (two rows share
+    // a word with 16-bit types), so 8 rows take 5 or 8 shuffles instead of 32, and each scale is computed by
+    // the threads that end up with its row.
+    constexpr int kPer = sizeof(T) == 2 ? 2 : 1;  // rows per word
+    constexpr int kHeld = 8 / kPer;
+    constexpr int kKeep = kPer == 2 ? 4 : 2;      // the last exchange that halves
+    const int lane = threadIdx.x & 31;
+    Scale mine[kPer];
+    if constexpr (!kBlock) {
+      uint32_t m[kHeld];
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        uint32_t row[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          row[e] = 0;
+#pragma unroll
+          for (int j = 0; j < kWords; ++j) row[e] = max_mag<T>(row[e], mag<T>(v[h * kPer + e].w[j]));
+        }
+        if constexpr (kPer == 2) m[h] = __vmaxu2(__byte_perm(row[0], row[1], 0x5410), __byte_perm(row[0], row[1], 0x7632));
+        else m[h] = row[0];
+      }
+#pragma unroll
+      for (int o = 8, left = kHeld; o >= 1; o /= 2) {
+        if (o >= kKeep) {
+          left /= 2;
+          const bool upper = (lane & o) != 0;
+#pragma unroll
+          for (int h = 0; h < kHeld / 2; ++h) {
+            if (h >= left) break;
+            const uint32_t keep = upper ? m[h + left] : m[h], give = upper ? m[h] : m[h + left];
+            m[h] = max_mag<T>(keep, __shfl_xor_sync(0xffffffffu, give, o));
+          }
+        } else {
+          m[0] = max_mag<T>(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
+        }
+      }
+      const int first = (kPer == 2 ? ((lane & 12) >> 2) : ((lane & 14) >> 1)) * kPer;  // the thread's first row
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        mine[e] = scale_of<kTop>(mag_bits<T>(e == 0 ? m[0] & (kPer == 2 ? 0xffffu : 0xffffffffu) : m[0] >> 16));
+        const int64_t r = row0 + first + e;
+        if ((lane & (kKeep - 1)) == 0 && r < p.rows) p.scale[r * p.scale_row + tc * p.scale_blk] = mine[e].s;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      Scale s = block_scale;
-      if constexpr (!kBlock) {
-        uint32_t amax = 0;
+      float inv = block_scale.inverse;
+      if constexpr (!kBlock) inv = __shfl_sync(0xffffffffu, mine[i % kPer].inverse, (lane & 16) | (i / kPer) * kKeep);
+      float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, abs_bits(v[i][j]));
-#pragma unroll
-        for (int o = 1; o < 16; o *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        s = scale_of<kTop>(amax);
-        if ((threadIdx.x & 15) == 0 && row0 + i < p.rows) p.scale[(row0 + i) * p.scale_row + tc * p.scale_blk] = s.s;
-      }
+      for (int j = 0; j < 8; ++j) f[j] = v[i].get(j);
       if (row0 + i < p.rows)
-        store8(p.q + (row0 + i) * p.ldq + col0, make_uint2(cvt4<kTop>(v[i], s.inverse), cvt4<kTop>(v[i] + 4, s.inverse)), n,
-               vec_q);
+        store8(p.q + (row0 + i) * p.ldq + col0, make_uint2(cvt4<kTop>(f, inv), cvt4<kTop>(f + 4, inv)), n, vec_q);
     }
   }
   if constexpr (kCols) {
-    if constexpr (!kBlock) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t amax = 0;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          amax = max(amax, abs_bits(v[i][j]));
-          sum += v[i][j];
-        }
-        col_amax[slot][c0 + j] = amax;
-        col_part[slot][c0 + j] = sum;
-      }
-      __syncthreads();
-      if (threadIdx.x < kGroup) {
-        uint32_t amax = 0;
-        float sum = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 16; ++s) {
-          amax = max(amax, col_amax[s][threadIdx.x]);
-          sum += col_part[s][threadIdx.x];
-        }
-        const Scale s = scale_of<kTop>(amax);
-        col_scale[threadIdx.x] = s;
-        const int64_t c = tc * kGroup + threadIdx.x;
-        if (c < p.cols) {
-          p.scale_t[c * p.scale_t_row + tr * p.scale_t_blk] = s.s;
-          if (p.col_sums != nullptr) p.col_sums[tr * p.cols + c] = sum;
-        }
-      }
-      __syncthreads();
-    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float inv = kBlock ? block_scale.inverse : col_scale[c0 + j].inverse;
-      float t[8];
+      const float inv = kBlock ? block_scale.inverse : col_inverse[c0 + j];
+      float f[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = v[i][j];
-      *reinterpret_cast<uint2*>(turned + (c0 + j) * kTilePitch + slot * 8) = make_uint2(cvt4<kTop>(t, inv), cvt4<kTop>(t + 4, inv));
+      for (int i = 0; i < 8; ++i) f[i] = v[i].get(j);
+      *reinterpret_cast<uint2*>(turned + (c0 + j) * kGroup + (((slot >> 1) ^ (threadIdx.x & 7)) << 4) + (slot & 1) * 8) =
+          make_uint2(cvt4<kTop>(f, inv), cvt4<kTop>(f + 4, inv));
     }
     __syncthreads();
     // 8 threads write one 128-byte row of the transposed tile, 32 rows at a time.
-    const int64_t r = tr * kGroup + (threadIdx.x & 7) * 16;
+    const int unit = threadIdx.x & 7;
+    const int64_t r = tr * kGroup + unit * 16;
     const int64_t left = p.rows - r;
 #pragma unroll
     for (int k = 0; k < kGroup; k += kTileThreads / 8) {
       const int c = k + (threadIdx.x >> 3);
       if (tc * kGroup + c >= p.cols) continue;
-      const uint4 b = *reinterpret_cast<const uint4*>(turned + c * kTilePitch + (threadIdx.x & 7) * 16);
+      const uint4 b = *reinterpret_cast<const uint4*>(turned + c * kGroup + ((unit ^ ((c >> 3) & 7)) << 4));
       uint8_t* dst = p.qt + (tc * kGroup + c) * p.ldqt + r;
       if (left >= 16 && vec_qt) {
         *reinterpret_cast<uint4*>(dst) = b;
