@@ -10,15 +10,18 @@
 //   torch.ops.zcutlass.linear(x, weight, bias=None) -> y
 //       nn.functional.linear semantics: weight is the PyTorch [N, K] layout and
 //       is consumed directly as a column-major B (no transposed copy).
-//   torch.ops.zcutlass.{quantize_fp8, gemm_fp8, linear_fp8, linear_fp8_forward,
-//       linear_fp8_backward, rotary, rotary_}  8-bit block-scaled linears and
+//   torch.ops.zcutlass.{quantize_fp8, gemm_fp8, linear_fp8, linear_fp8_train,
+//       rotary, rotary_}  8-bit block-scaled linears and
 //       rotary positions over the C ABI (documented in torch_ops.py)
 //
 // This file only adapts tensors to the library's entry points; all kernels live in libzcutlass.so.
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
@@ -172,23 +175,36 @@ int32_t fp8_code(at::ScalarType t, const char* name) {
 constexpr int64_t kFp8Group = 128;
 int64_t groups(int64_t n) { return (n + kFp8Group - 1) / kFp8Group; }
 
-// Row stride of a matrix whose rows are contiguous (one row or no values: any).
+// Row stride of a matrix whose rows are contiguous (one row or no values: any; a multiple of 16 then).
 int64_t row_stride(const at::Tensor& t, const char* name) {
-  if (t.numel() == 0) return std::max<int64_t>(t.size(1), 1);
+  const int64_t any = (std::max<int64_t>(t.size(1), 1) + 15) / 16 * 16;
+  if (t.numel() == 0) return any;
   TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " must have contiguous rows");
-  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), name, " must not have overlapping rows");
-  return t.size(0) <= 1 ? std::max<int64_t>(t.size(1), 1) : t.stride(0);
+  if (t.size(0) == 1) return any;
+  TORCH_CHECK(t.stride(0) >= t.size(1), name, " must not have overlapping rows");
+  return t.stride(0);
+}
+
+// New tensors straight from the caching allocator: what these calls run on is often a few microseconds of
+// kernel, so the dispatcher's share of at::empty and of the views after it would be most of the call.
+at::Tensor empty_like_device(at::IntArrayRef sizes, at::ScalarType t, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, t, like.device(), std::nullopt));
 }
 
 // An 8-bit matrix with rows padded to 16 bytes (what TMA can describe).
 at::Tensor empty_fp8(int64_t rows, int64_t cols, at::ScalarType t, const at::Tensor& like) {
   const int64_t ld = (cols + 15) / 16 * 16;
-  return at::empty({rows, ld}, like.options().dtype(t)).narrow(1, 0, cols);
+  at::Tensor q = empty_like_device({rows, ld}, t, like);
+  q.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({rows, cols}), at::IntArrayRef({ld, int64_t(1)}));
+  return q;
 }
 
 // Scales [rows, groups], rows contiguous: the product's kernels read the scales of neighbouring rows together.
 at::Tensor empty_row_scales(int64_t rows, int64_t cols, const at::Tensor& like) {
-  return at::empty({groups(cols), rows}, like.options().dtype(at::kFloat)).t();
+  at::Tensor s = empty_like_device({groups(cols), rows}, at::kFloat, like);
+  s.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({rows, groups(cols)}),
+                                                 at::IntArrayRef({int64_t(1), std::max<int64_t>(rows, 1)}));
+  return s;
 }
 
 struct Quantized {
@@ -201,18 +217,17 @@ Quantized quantize(const at::Tensor& x, bool rows, bool columns, int64_t block_r
   zcutlass_quantize_desc d{};
   d.rows = m, d.cols = n, d.ldx = row_stride(x, "x");
   d.x_type = float_code(x, "x"), d.q_type = fp8_code(type, "dtype"), d.block_rows = static_cast<int32_t>(block_rows);
-  const auto f32 = x.options().dtype(at::kFloat);
   if (rows) {
     r.q = empty_fp8(m, n, type, x);
-    r.scale = block_rows == 1 ? empty_row_scales(m, n, x) : at::empty({groups(m), groups(n)}, f32);
+    r.scale = block_rows == 1 ? empty_row_scales(m, n, x) : empty_like_device({groups(m), groups(n)}, at::kFloat, x);
     d.ldq = r.q.stride(0), d.scale_row = r.scale.stride(0), d.scale_blk = r.scale.stride(1);
   }
   if (columns) {
     r.qt = empty_fp8(n, m, type, x);
-    r.scale_t = block_rows == 1 ? empty_row_scales(n, m, x) : at::empty({groups(n), groups(m)}, f32);
+    r.scale_t = block_rows == 1 ? empty_row_scales(n, m, x) : empty_like_device({groups(n), groups(m)}, at::kFloat, x);
     d.ldqt = r.qt.stride(0), d.scale_t_row = r.scale_t.stride(0), d.scale_t_blk = r.scale_t.stride(1);
   }
-  if (sums) r.col_sums = at::empty({groups(m), n}, f32);
+  if (sums) r.col_sums = empty_like_device({groups(m), n}, at::kFloat, x);
   d.stream = current_stream();
   const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
   check_status(zcutlass_quantize_fp8(&d, x.data_ptr(), ptr(r.q), static_cast<float*>(ptr(r.scale)), ptr(r.qt),
@@ -259,9 +274,10 @@ void check_fp8_operand(const at::Tensor& t, const at::Tensor& scale, const char*
 }
 
 at::Tensor run_gemm_fp8(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale,
-                        const std::optional<at::Tensor>& bias, at::ScalarType out_type) {
+                        const std::optional<at::Tensor>& bias, at::ScalarType out_type,
+                        at::IntArrayRef shape = {}) {
   const int64_t m = a.size(0), n = b.size(0), k = a.size(1);
-  at::Tensor d = at::empty({m, n}, a.options().dtype(out_type));
+  at::Tensor d = shape.empty() ? empty_like_device({m, n}, out_type, a) : empty_like_device(shape, out_type, a);
   zcutlass_fp8_gemm_desc g{};
   g.m = m, g.n = n, g.k = k;
   g.lda = row_stride(a, "A"), g.ldb = row_stride(b, "B"), g.ldd = n;
@@ -298,7 +314,7 @@ at::Tensor gemm_fp8_op(const at::Tensor& a, const at::Tensor& a_scale, const at:
 at::Tensor as_rows(const at::Tensor& x) {
   int64_t rows = 1;
   for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
-  const at::Tensor x2 = x.reshape({rows, x.size(-1)});
+  const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({rows, x.size(-1)});
   const bool ok = (x2.size(1) <= 1 || x2.stride(1) == 1) && (rows <= 1 || x2.stride(0) >= x2.size(1));
   return ok ? x2 : x2.contiguous();
 }
@@ -314,13 +330,17 @@ at::Tensor linear_fp8_op(const at::Tensor& x, const at::Tensor& w, const at::Ten
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = w.size(0);
   const Quantized r = quantize(as_rows(x), true, false, 1, at::kFloat8_e4m3fn, false);
-  return run_gemm_fp8(r.q, r.scale, w, w_scale, bias, x.scalar_type()).view(shape);
+  return run_gemm_fp8(r.q, r.scale, w, w_scale, bias, x.scalar_type(), shape);
 }
 
-// The differentiable linear: y, then what its backward pass needs of x and w, each in 8 bits and
-// transposed (undefined where the gradient it serves is not wanted).
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_fp8_forward_op(
-    const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, bool need_dx, bool need_dw) {
+// The differentiable linear keeps x and w in 8 bits, transposed, for its backward pass (undefined where the
+// gradient they serve is not wanted).
+struct LinearKept {
+  at::Tensor y, wt, wt_scale, xt, xt_scale;
+};
+
+LinearKept linear_fp8_forward(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, bool need_dx,
+                              bool need_dw) {
   TORCH_CHECK(x.is_cuda() && x.dim() >= 1, "x must be a CUDA tensor");
   TORCH_CHECK(w.is_cuda() && w.dim() == 2, "weight must be a rank-2 CUDA tensor");
   TORCH_CHECK(x.device() == w.device(), "x and weight must be on the same CUDA device");
@@ -330,38 +350,38 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_fp
   shape.back() = w.size(0);
   const Quantized qx = quantize(as_rows(x), true, need_dw, 1, at::kFloat8_e4m3fn, false);
   const Quantized qw = quantize(as_rows(w), true, need_dx, kFp8Group, at::kFloat8_e4m3fn, false);
-  const at::Tensor y = run_gemm_fp8(qx.q, qx.scale, qw.q, qw.scale, bias, x.scalar_type()).view(shape);
-  const at::Tensor none = at::empty({0}, x.options());
-  return {y, need_dx ? qw.qt : none, need_dx ? qw.scale_t : none, need_dw ? qx.qt : none, need_dw ? qx.scale_t : none};
+  return {run_gemm_fp8(qx.q, qx.scale, qw.q, qw.scale, bias, x.scalar_type(), shape), qw.qt, qw.scale_t, qx.qt, qx.scale_t};
 }
 
-// dx = Q(dy) Q(w), dw = Q(dy^T) Q(x^T)^T, db = column sums of dy; empty tensors where not wanted.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_fp8_backward_op(
-    const at::Tensor& grad, const at::Tensor& wt, const at::Tensor& wt_scale, const at::Tensor& xt, const at::Tensor& xt_scale,
-    bool need_dx, bool need_dw, bool need_db, at::ScalarType dw_dtype) {
-  TORCH_CHECK(grad.is_cuda() && grad.dim() >= 1, "dy must be a CUDA tensor");
+struct LinearGrads {
+  at::Tensor dx, dw, db;
+};
+
+// dx = Q(dy) Q(w), dw = Q(dy^T) Q(x^T)^T, db = column sums of dy; undefined where not wanted.
+LinearGrads linear_fp8_backward(const at::Tensor& grad, const at::Tensor& wt, const at::Tensor& wt_scale, const at::Tensor& xt,
+                                const at::Tensor& xt_scale, bool need_dx, bool need_dw, bool need_db, at::ScalarType dw_dtype) {
+  LinearGrads g;
+  if (!need_dx && !need_dw && !need_db) return g;
   const c10::cuda::CUDAGuard guard(grad.device());
   const at::Tensor dy = as_rows(grad);
-  at::Tensor dx = at::empty({0}, dy.options()), dw = dx, db = dx;
-  if (!need_dx && !need_dw && !need_db) return {dx, dw, db};
   const Quantized r = quantize(dy, need_dx, need_dw || need_db, 1, at::kFloat8_e4m3fn, need_db);
   if (need_dx) {
-    check_fp8_operand(wt, wt_scale, "weight", true);
     std::vector<int64_t> shape(grad.sizes().begin(), grad.sizes().end());
     shape.back() = wt.size(0);
-    dx = run_gemm_fp8(r.q, r.scale, wt, wt_scale, std::nullopt, dy.scalar_type()).view(shape);
+    g.dx = run_gemm_fp8(r.q, r.scale, wt, wt_scale, std::nullopt, dy.scalar_type(), shape);
   }
-  if (need_dw) {
-    check_fp8_operand(xt, xt_scale, "x", true);
-    dw = run_gemm_fp8(r.qt, r.scale_t, xt, xt_scale, std::nullopt, dw_dtype);
-  }
+  if (need_dw) g.dw = run_gemm_fp8(r.qt, r.scale_t, xt, xt_scale, std::nullopt, dw_dtype);
   if (need_db) {
-    db = at::empty({dy.size(1)}, dy.options());
-    check_status(zcutlass_sum_rows(r.col_sums.data_ptr<float>(), r.col_sums.size(0), dy.size(1), db.data_ptr(),
-                                   float_code(db, "dy"), current_stream()),
+    g.db = empty_like_device({dy.size(1)}, dy.scalar_type(), dy);
+    check_status(zcutlass_sum_rows(r.col_sums.data_ptr<float>(), r.col_sums.size(0), dy.size(1), g.db.data_ptr(),
+                                   float_code(g.db, "dy"), current_stream()),
                  "zcutlass_sum_rows");
   }
-  return {dx, dw, db};
+  return g;
+}
+
+at::Tensor linear_fp8_train_op(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias) {
+  return linear_fp8_forward(x, w, bias, false, false).y;
 }
 
 // ---------------------------------------------------------------- rotary positions
@@ -408,7 +428,8 @@ void run_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_ou
 std::tuple<at::Tensor, at::Tensor> rotary_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                                              const at::Tensor& table, bool interleaved, bool inverse) {
   const c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor q_out = at::empty(q.sizes(), q.options()), k_out = at::empty(k.sizes(), k.options());
+  TORCH_CHECK(q.is_cuda() && k.is_cuda(), "q and k must be CUDA tensors");
+  at::Tensor q_out = empty_like_device(q.sizes(), q.scalar_type(), q), k_out = empty_like_device(k.sizes(), k.scalar_type(), k);
   run_rotary(q, k, q_out, k_out, positions, table, interleaved, inverse);
   return {q_out, k_out};
 }
@@ -422,17 +443,140 @@ void rotary_inplace_op(at::Tensor q, at::Tensor k, const at::Tensor& positions, 
   run_rotary(q, k, q, k, positions, table, interleaved, inverse);
 }
 
+// ---------------------------------------------------------------- gradients
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+
 // While the current stream is being captured: refuses a leaf whose gradient accumulator was made on another
 // stream and is still alive (an eager graph of the same leaf is). The backward pass would wait for that
 // stream, which ends the capture, or the process.
-void check_capture_op(const at::Tensor& leaf) {
-  if (!leaf.requires_grad() || leaf.grad_fn() != nullptr) return;
+void check_capture(const at::Tensor& leaf) {
+  if (!wants_grad(leaf) || !leaf.is_cuda() || leaf.grad_fn() != nullptr) return;
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
   if (accumulator == nullptr) return;
   const auto made_on = accumulator->stream();
   TORCH_CHECK(!made_on.has_value() || *made_on == at::cuda::getCurrentCUDAStream(leaf.get_device()).unwrap(),
               "a graph of this leaf made on another stream is still alive: drop it (its outputs and losses) before "
               "capturing a backward pass");
+}
+
+template <typename... T>
+void check_no_gradient(const char* name, const T&... t) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(t) || ...), name,
+              " has no gradient: use linear_fp8_train, or call it under torch.no_grad()");
+}
+
+class LinearFp8 : public torch::autograd::Function<LinearFp8> {
+ public:
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const std::optional<at::Tensor>& bias, bool need_dx, bool need_dw, bool need_db) {
+    const at::AutoDispatchBelowADInplaceOrView guard;
+    const LinearKept kept = linear_fp8_forward(x, w, bias, need_dx, need_dw);
+    ctx->save_for_backward({kept.wt, kept.wt_scale, kept.xt, kept.xt_scale});
+    ctx->saved_data["w"] = static_cast<int64_t>(w.scalar_type());
+    ctx->saved_data["need"] = static_cast<int64_t>((need_dx ? 1 : 0) | (need_dw ? 2 : 0) | (need_db ? 4 : 0));
+    return kept.y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "linear_fp8_train has no second derivative (create_graph)");
+    variable_list out(6);
+    if (!grads[0].defined()) return out;
+    const int64_t need = ctx->saved_data["need"].toInt();
+    const auto kept = ctx->get_saved_variables();
+    // Of the gradients that the operands allow, those that this backward pass asks for.
+    LinearGrads g = linear_fp8_backward(grads[0], kept[0], kept[1], kept[2], kept[3],
+                                        (need & 1) != 0 && ctx->needs_input_grad(0), (need & 2) != 0 && ctx->needs_input_grad(1),
+                                        (need & 4) != 0 && ctx->needs_input_grad(2),
+                                        static_cast<at::ScalarType>(ctx->saved_data["w"].toInt()));
+    out[0] = std::move(g.dx), out[1] = std::move(g.dw), out[2] = std::move(g.db);
+    return out;
+  }
+};
+
+at::Tensor linear_fp8_train_autograd(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias) {
+  const at::Tensor b = bias.value_or(at::Tensor());
+  if (!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || wants_grad(b))) {
+    const at::AutoDispatchBelowADInplaceOrView guard;
+    return linear_fp8_train_op(x, w, bias);
+  }
+  check_capture(x);
+  check_capture(w);
+  check_capture(b);
+  return LinearFp8::apply(x, w, bias, wants_grad(x), wants_grad(w), wants_grad(b));
+}
+
+class Rotary : public torch::autograd::Function<Rotary> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                               const at::Tensor& table, bool interleaved, bool inverse) {
+    const at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->save_for_backward({positions, table});
+    ctx->saved_data["mode"] = static_cast<int64_t>((interleaved ? 1 : 0) | (inverse ? 2 : 0));
+    auto [qo, ko] = rotary_op(q, k, positions, table, interleaved, inverse);
+    return {std::move(qo), std::move(ko)};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads);
+};
+
+std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                                                   const at::Tensor& table, bool interleaved, bool inverse) {
+  if (!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k))) {
+    const at::AutoDispatchBelowADInplaceOrView guard;
+    return rotary_op(q, k, positions, table, interleaved, inverse);
+  }
+  check_capture(q);
+  check_capture(k);
+  variable_list out = Rotary::apply(q, k, positions, table, interleaved, inverse);
+  return {std::move(out[0]), std::move(out[1])};
+}
+
+// The map is linear, its gradient the rotation back: differentiable itself.
+variable_list Rotary::backward(AutogradContext* ctx, variable_list grads) {
+  const auto kept = ctx->get_saved_variables();
+  const int64_t mode = ctx->saved_data["mode"].toInt();
+  for (at::Tensor& g : grads)
+    if (g.size(2) > 1 && g.stride(2) != 1) g = g.contiguous();
+  auto [dq, dk] = rotary_autograd(grads[0], grads[1], kept[0], kept[1], (mode & 1) != 0, (mode & 2) == 0);
+  variable_list out(6);
+  out[0] = std::move(dq), out[1] = std::move(dk);
+  return out;
+}
+
+std::vector<at::Tensor> quantize_fp8_autograd(const at::Tensor& x, std::string_view layout, std::optional<at::ScalarType> dtype) {
+  check_no_gradient("quantize_fp8", x);
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return quantize_fp8_op(x, layout, dtype);
+}
+
+at::Tensor gemm_fp8_autograd(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale,
+                             const std::optional<at::Tensor>& bias, std::optional<at::ScalarType> out_dtype) {
+  check_no_gradient("gemm_fp8", a_scale, b_scale, bias.value_or(at::Tensor()));
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return gemm_fp8_op(a, a_scale, b, b_scale, bias, out_dtype);
+}
+
+at::Tensor linear_fp8_autograd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
+                               const std::optional<at::Tensor>& bias) {
+  check_no_gradient("linear_fp8", x, w_scale, bias.value_or(at::Tensor()));
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return linear_fp8_op(x, w, w_scale, bias);
+}
+
+void rotary_inplace_autograd(at::Tensor q, at::Tensor k, const at::Tensor& positions, const at::Tensor& table,
+                             bool interleaved, bool inverse) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k)),
+              "rotary_ has no gradient: use rotary, or call it under torch.no_grad()");
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  rotary_inplace_op(q, k, positions, table, interleaved, inverse);
+  // Saved for a backward pass elsewhere, the old values are gone: let autograd see it.
+  q.unsafeGetTensorImpl()->bump_version();
+  k.unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace
@@ -450,15 +594,11 @@ TORCH_LIBRARY(zcutlass, m) {
   m.def("quantize_fp8(Tensor x, str layout=\"rows\", ScalarType? dtype=None) -> Tensor[]");
   m.def("gemm_fp8(Tensor A, Tensor A_scale, Tensor B, Tensor B_scale, Tensor? bias=None, ScalarType? out_dtype=None) -> Tensor");
   m.def("linear_fp8(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias=None) -> Tensor");
-  m.def("linear_fp8_forward(Tensor x, Tensor weight, Tensor? bias, bool need_dx, bool need_dw) -> "
-        "(Tensor, Tensor, Tensor, Tensor, Tensor)");
-  m.def("linear_fp8_backward(Tensor dy, Tensor weight_t, Tensor weight_t_scale, Tensor x_t, Tensor x_t_scale, "
-        "bool need_dx, bool need_dw, bool need_db, ScalarType dw_dtype) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_fp8_train(Tensor x, Tensor weight, Tensor? bias=None) -> Tensor");
   m.def("rotary(Tensor q, Tensor k, Tensor positions, Tensor table, bool interleaved=False, bool inverse=False) -> "
         "(Tensor, Tensor)");
   m.def("rotary_(Tensor(a!) q, Tensor(b!) k, Tensor positions, Tensor table, bool interleaved=False, "
         "bool inverse=False) -> ()");
-  m.def("check_capture(Tensor leaf) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(zcutlass, CUDA, m) {
@@ -468,9 +608,16 @@ TORCH_LIBRARY_IMPL(zcutlass, CUDA, m) {
   m.impl("quantize_fp8", quantize_fp8_op);
   m.impl("gemm_fp8", gemm_fp8_op);
   m.impl("linear_fp8", linear_fp8_op);
-  m.impl("linear_fp8_forward", linear_fp8_forward_op);
-  m.impl("linear_fp8_backward", linear_fp8_backward_op);
+  m.impl("linear_fp8_train", linear_fp8_train_op);
   m.impl("rotary", rotary_op);
   m.impl("rotary_", rotary_inplace_op);
-  m.impl("check_capture", check_capture_op);
+}
+
+TORCH_LIBRARY_IMPL(zcutlass, Autograd, m) {
+  m.impl("quantize_fp8", quantize_fp8_autograd);
+  m.impl("gemm_fp8", gemm_fp8_autograd);
+  m.impl("linear_fp8", linear_fp8_autograd);
+  m.impl("linear_fp8_train", linear_fp8_train_autograd);
+  m.impl("rotary", rotary_autograd);
+  m.impl("rotary_", rotary_inplace_autograd);
 }

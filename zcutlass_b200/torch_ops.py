@@ -138,11 +138,13 @@ def linear(x, weight, bias=None):
 # ---------------------------------------------------------------- 8-bit linears
 
 
-def _no_gradient(name: str, *tensors) -> None:
+@functools.cache
+def _op(name: str):
+    """The registered operator (its only overload: a call on it skips the overload search)."""
     import torch
 
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no gradient: use linear_fp8_train, or call it under torch.no_grad()")
+    load()
+    return getattr(torch.ops.zcutlass, name).default
 
 
 def quantize_fp8(x, layout: str = "rows", dtype=None) -> tuple:
@@ -161,11 +163,7 @@ def quantize_fp8(x, layout: str = "rows", dtype=None) -> tuple:
     rounded to nearest even. A group with an infinity or a NaN becomes NaN
     throughout, its scale too. Rows of q are padded to 16 bytes in memory
     (stride), as gemm_fp8 reads them fastest."""
-    import torch
-
-    load()
-    _no_gradient("quantize_fp8", x)
-    return tuple(torch.ops.zcutlass.quantize_fp8(x, layout, dtype))
+    return tuple(_op("quantize_fp8")(x, layout, dtype))
 
 
 def gemm_fp8(a, a_scale, b, b_scale, bias=None, out_dtype=None):
@@ -176,11 +174,7 @@ def gemm_fp8(a, a_scale, b, b_scale, bias=None, out_dtype=None):
     a_scale [M, ceil(K / 128)]; b_scale [N, ceil(K / 128)], or
     [ceil(N / 128), ceil(K / 128)] for weights in 128 x 128 blocks: float32 of
     any value and any strides."""
-    import torch
-
-    load()
-    _no_gradient("gemm_fp8", a_scale, b_scale, bias)
-    return torch.ops.zcutlass.gemm_fp8(a, a_scale, b, b_scale, bias, out_dtype)
+    return _op("gemm_fp8")(a, a_scale, b, b_scale, bias, out_dtype)
 
 
 def linear_fp8(x, weight, weight_scale, bias=None):
@@ -188,47 +182,7 @@ def linear_fp8(x, weight, weight_scale, bias=None):
     (quantize_fp8(w, "blocks"), or a checkpoint's values and scales) and x
     quantised by rows on the way in; y has x's dtype. For serving; training
     uses linear_fp8_train."""
-    import torch
-
-    load()
-    _no_gradient("linear_fp8", x, weight_scale, bias)
-    return torch.ops.zcutlass.linear_fp8(x, weight, weight_scale, bias)
-
-
-def _check_capture(*tensors) -> None:
-    """Under stream capture: refuses leaves that an eager graph made on another stream still holds, whose
-    backward pass would end the capture (or the process)."""
-    import torch
-
-    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
-        for t in tensors:
-            if t is not None and t.is_cuda and t.requires_grad:
-                torch.ops.zcutlass.check_capture(t)
-
-
-@functools.cache
-def _linear_fp8_function():
-    import torch
-    from torch.autograd.function import once_differentiable
-
-    class LinearFp8(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, weight, bias):
-            need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-            y, *kept = torch.ops.zcutlass.linear_fp8_forward(x, weight, bias, need_dx, need_dw)
-            ctx.save_for_backward(*kept)
-            ctx.weight_dtype = weight.dtype
-            return y
-
-        @staticmethod
-        @once_differentiable
-        def backward(ctx, dy):
-            need_dx, need_dw, need_db = ctx.needs_input_grad
-            dx, dw, db = torch.ops.zcutlass.linear_fp8_backward(dy, *ctx.saved_tensors, need_dx, need_dw, need_db,
-                                                                ctx.weight_dtype)
-            return dx if need_dx else None, dw if need_dw else None, db if need_db else None
-
-    return LinearFp8
+    return _op("linear_fp8")(x, weight, weight_scale, bias)
 
 
 def linear_fp8_train(x, weight, bias=None):
@@ -244,9 +198,7 @@ def linear_fp8_train(x, weight, bias=None):
     x, bias: one of float16, bfloat16, float32; weight: any of them. The
     backward pass keeps x and weight in 8 bits only. Capturing a step into a
     CUDA graph is refused while an eager graph of the same leaves is alive."""
-    load()
-    _check_capture(x, weight, bias)
-    return _linear_fp8_function().apply(x, weight, bias)
+    return _op("linear_fp8_train")(x, weight, bias)
 
 
 # ---------------------------------------------------------------- rotary positions
@@ -324,29 +276,6 @@ def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, scaling
     return table
 
 
-@functools.cache
-def _rotary_function():
-    import torch
-    from torch.autograd.function import once_differentiable
-
-    class Rotary(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, q, k, positions, table, interleaved):
-            ctx.save_for_backward(positions, table)
-            ctx.interleaved = interleaved
-            return torch.ops.zcutlass.rotary(q, k, positions, table, interleaved)
-
-        @staticmethod
-        @once_differentiable
-        def backward(ctx, dq, dk):
-            positions, table = ctx.saved_tensors
-            dq, dk = (g if g.shape[-1] <= 1 or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk))
-            dq, dk = torch.ops.zcutlass.rotary(dq, dk, positions, table, ctx.interleaved, True)
-            return dq, dk, None, None, None
-
-    return Rotary
-
-
 def rotary(q, k, positions, table, interleaved: bool = False):
     """Rotary positions on q [tokens, q_heads, head_dim] and k [tokens,
     k_heads, head_dim] (float16, bfloat16 or float32, any token and head
@@ -359,20 +288,13 @@ def rotary(q, k, positions, table, interleaved: bool = False):
     A negative position marks padding, whose heads are copied as they are. A
     position at or beyond the table's end does the same and sets the device
     error word (zcutlass_b200.tp.check_device_error raises on it)."""
-    import torch
-
-    load()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-        _check_capture(q, k)
-        return _rotary_function().apply(q, k, positions, table, interleaved)
-    return torch.ops.zcutlass.rotary(q, k, positions, table, interleaved)
+    return _op("rotary")(q, k, positions, table, interleaved)
 
 
 def rotary_(q, k, positions, table, interleaved: bool = False) -> None:
     """rotary() in place, without gradients."""
     import torch
 
-    load()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
         raise RuntimeError("rotary_ has no gradient: use rotary, or call it under torch.no_grad()")
-    torch.ops.zcutlass.rotary_(q, k, positions, table, interleaved)
+    _op("rotary_")(q, k, positions, table, interleaved)
