@@ -127,7 +127,7 @@ def test_gemm_types(cuda_device, mnk, fa, fb):
     check_gemm(a, sa, b, sb, F16)
 
 
-KERNELS = ["fp8_generic", "fp8_swap16", "fp8_swap32", "fp8_swap64", "fp8_swap128", "fp8_pair"]
+KERNELS = ["fp8_generic", "fp8_tile16", "fp8_tile32", "fp8_tile64", "fp8_tile128", "fp8_pair"]
 
 
 @pytest.mark.parametrize("b_rows", [False, True], ids=["b_blocks", "b_rows"])

@@ -59,6 +59,17 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
+// 16 rows x 8 columns of 32 bits per 4 registers: registers 4 g, 4 g + 1 hold columns 8 g + (lane % 4) * 2
+// and the next of row lane / 4, registers 4 g + 2, 4 g + 3 the same of row lane / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
 // Waits for the thread's TMEM loads; the registers pass through so that no use of them moves above the wait.
 __device__ __forceinline__ void tmem_ld_wait_x16(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -90,44 +101,6 @@ __device__ __forceinline__ bool elect_one() {
 // scope it waits for every load in flight, the scales fetched ahead among them (4x slower per block).
 __device__ __forceinline__ void arrive_read(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
-// Two 32-bit values in one register pair.
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  return v;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  uint32_t lo, hi;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
-}
-__device__ __forceinline__ uint64_t both(float v) { return pack2(__float_as_uint(v), __float_as_uint(v)); }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
-}
-
-// Barrier kId of kThreads threads that also tells every one of them whether all passed true.
-template <int kId, int kThreads>
-__device__ __forceinline__ bool barrier_and(bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n"
-      " .reg .pred p, q;\n"
-      " setp.ne.b32 p, %3, 0;\n"
-      " barrier.cta.red.and.pred q, %1, %2, p;\n"
-      " selp.u32 %0, 1, 0, q;\n"
-      "}\n"
-      : "=r"(r)
-      : "n"(kId), "n"(kThreads), "r"(ok ? 1 : 0)
-      : "memory");
-  return r != 0;
 }
 
 // Four floats at a shared-memory offset of another CTA of the cluster.

@@ -104,17 +104,6 @@ __device__ __forceinline__ void raster(int tile, const Fp8PairParams& p, int& tm
   tn = in / rows;
 }
 
-// 16 rows x 8 columns of 32 bits per 4 registers: registers 4 g, 4 g + 1 hold columns 8 g + (lane % 4) * 2
-// and the next of row lane / 4, registers 4 g + 2, 4 g + 3 the same of row lane / 4 + 8.
-__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
 template <bool kRows>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -341,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(scale, __uint_as_float(r[j]), acc[c * 16 + j]);
           }
         } else {
-          tmem_ld_16x256b_x4(t0, v[0]);
+          fp8::tmem_ld_16x256b_x4(t0, v[0]);
           float sa[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) sa[j] = slot[quarter * 32 + j * 8 + (lane >> 2)];
@@ -351,11 +340,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t(&r)[16] = v[c & 1];
             fp8::tmem_ld_wait_x16(r);
             if (c + 1 < 8) {
-              tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, v[(c + 1) & 1]);
+              fp8::tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, v[(c + 1) & 1]);
             } else {
               tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
             }
             const float lo = sa[2 * (c & 1)], hi = sa[2 * (c & 1) + 1];
 #pragma unroll
@@ -368,6 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               q[3] = fmaf(s.y * hi, __uint_as_float(r[4 * g + 3]), q[3]);
             }
           }
+          __syncwarp();  // the slot has been read, too
+          if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
         }
       }
       if (!ok) break;

@@ -1,0 +1,398 @@
+// 8-bit block-scaled product with one output tile per cluster of CTAs along K:
+// few rows of A (decode) and products too small for the pair kernel's tiles.
+//
+//   D[m, n] = sum_b sa(m, b) * sb(n, b) * (A_b B_b^T)[m, n]  (+ bias[n])
+//
+// kSwap (M <= 64): B's rows (weights) fill the 128-row MMA dimension and TM =
+// 16, 32 or 64 rows of A sit on MMA-N, so the tensor core reads no padding of
+// 128 rows and the weights, which are the bytes, are streamed once. Else A's
+// rows are on MMA-M and the tile is 128 x 128.
+//
+// Per block of 128 k, 4 MMAs fill one of four TMEM buffers; the four
+// accumulation warps (a TMEM lane per thread) add it, scaled, to 32-bit
+// accumulators in registers. As in the pair kernel, the MMA warp keeps its state
+// in uniform registers, and two warps stage each block's scales in shared
+// memory and complete the buffer's barrier together with the commit. With one
+// weight scale per 128 rows of B the staged value is the whole factor.
+// With a scale per row of B (kRows) it is a factor per thread (kSwap), or TMEM is
+// read as 16 x 8 fragments, in which a thread meets 32 of 128 columns.
+//
+// Bound by bytes: a stage of the TMA ring holds KSUB blocks. The splits' 32-bit
+// partial tiles are added in split order through distributed shared memory, so
+// the result does not depend on timing.
+#pragma once
+
+#include "sm100_fp8_common.cuh"
+
+namespace zcb {
+
+struct Fp8TileParams {
+  int m, n, num_kb, splits, tiles_m;
+  const float* a_scale;
+  int64_t a_scale_row, a_scale_blk;
+  const float* b_scale;
+  int64_t b_scale_row, b_scale_blk;
+  void* d;
+  int64_t ldd;
+  int d_type;
+  bool vec_d;  // four consecutive n of D may be stored at once
+  const void* bias;
+  uint32_t idesc;
+  int* error_word;
+};
+
+namespace fp8_tile {
+
+using fp8::kBlockK;
+constexpr int kBlockN = 128;
+constexpr int kThreads = 256;
+constexpr int kAccThreads = 128;
+constexpr int kMaxSplits = 8;
+constexpr int kBufs = 4;   // TMEM buffers
+constexpr int kSlots = 8;  // blocks whose scales are in shared memory
+
+template <bool kSwap, int TM, bool kRows, int STAGES, int KSUB>
+struct Smem {
+  static_assert(kSwap ? (TM == 16 || TM == 32 || TM == 64) : TM == 128, "");
+  static constexpr int kMmaN = kSwap ? TM : kBlockN;
+  static constexpr int kABytes = TM * kBlockK;
+  static constexpr int kBBytes = kBlockN * kBlockK;
+  static constexpr int kSub = kABytes + kBBytes;  // B first: both start on 1024 bytes
+  static constexpr int kStageBytes = KSUB * kSub;
+  static constexpr int kRedBytes = TM * kBlockN * 4;  // the partial tile [m][n], over the drained ring
+  static constexpr int kRing = STAGES * kStageBytes > kRedBytes ? STAGES * kStageBytes : kRedBytes;
+  static constexpr int kSlotFloats = TM + (kRows ? kBlockN : 0);
+  static constexpr int kScaleOff = kRing;
+  static constexpr int kBarOff = kScaleOff + kSlots * kSlotFloats * 4;
+  static constexpr int kNumBars = 2 * STAGES + 2 * kBufs + 1;
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kDynamicBytes = kMiscOff + 16 + 1024;
+  static constexpr uint32_t kTmemCols = kBufs * kMmaN;
+  static_assert(kSub % 1024 == 0 && kABytes % 1024 == 0 && kDynamicBytes <= 232448, "");
+};
+
+enum : int {
+  kErrProducerEmpty = (33 << 4) | 1,
+  kErrMmaFull = (33 << 4) | 2,
+  kErrMmaTmemEmpty = (33 << 4) | 3,
+  kErrAccTmemFull = (33 << 4) | 4,
+  kErrScaleTmemFull = (33 << 4) | 5,
+};
+
+// Partial tile element (m, 4 g): rows rotate their 16-byte units where a thread writes a whole row.
+template <bool kSwap>
+__device__ __forceinline__ int red_at(int m, int g) {
+  return m * kBlockN + 4 * (kSwap ? g : g ^ (m & 7));
+}
+
+template <bool kSwap, int TM, bool kRows, int STAGES, int KSUB>
+__global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                const Fp8TileParams p) {
+  using L = Smem<kSwap, TM, kRows, STAGES, KSUB>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tmem_full = empty + STAGES;
+  uint64_t* tmem_empty = tmem_full + kBufs;
+  uint64_t* drain = tmem_empty + kBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
+  float* const slots = reinterpret_cast<float*>(smem + L::kScaleOff);
+  float* const red = reinterpret_cast<float*>(smem);
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int split = static_cast<int>(blockIdx.x % p.splits);  // the cluster rank: clusters are `splits` wide
+  const int tile = static_cast<int>(blockIdx.x / p.splits);
+  const int m0 = (tile % p.tiles_m) * TM, n0 = (tile / p.tiles_m) * kBlockN;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(split) * p.num_kb / p.splits);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(split + 1) * p.num_kb / p.splits);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < kBufs; ++b) {
+      mbar_init(&tmem_full[b], 2);  // the commit and the scales
+      mbar_init(&tmem_empty[b], kAccThreads / 32);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, L::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+  const WaitCtx ctx{abort_flag, p.error_word};
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // B is read once when one tile of rows covers M; A by every CTA.
+      const uint64_t b_policy = p.tiles_m == 1 ? l2_policy_evict_first() : l2_policy_evict_last();
+      const uint64_t a_policy = l2_policy_evict_last();
+      uint32_t it = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; kb += KSUB, ++it) {
+        const uint32_t s = it % STAGES;
+        if (!fp8::wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, ctx, kErrProducerEmpty)) {
+          ok = false;
+          break;
+        }
+        const int subs = kb1 - kb < KSUB ? kb1 - kb : KSUB;
+        mbar_arrive_expect_tx(&full[s], subs * L::kSub);
+#pragma unroll
+        for (int sub = 0; sub < KSUB; ++sub) {
+          if (sub >= subs) break;
+          uint8_t* at = smem + s * L::kStageBytes + sub * L::kSub;
+          tma_load_2d_hint(at, &tmap_b, &full[s], (kb + sub) * kBlockK, n0, b_policy);
+          tma_load_2d_hint(at + L::kBBytes, &tmap_a, &full[s], (kb + sub) * kBlockK, m0, a_policy);
+        }
+      }
+      if (!ok) {  // loads already issued must land before the CTA can exit
+        const uint32_t first = it > static_cast<uint32_t>(STAGES) ? it - STAGES : 0u;
+        for (uint32_t j = first; j < it; ++j) mbar_wait_quiet(&full[j % STAGES], (j / STAGES) & 1u, 200000000ull);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const bool one = fp8::elect_one();
+    uint32_t s = 0, phase = 0, buf = 0, buf_phase = 1;
+    bool ok = true, issued = false;
+    const uint64_t desc0 = smem_desc_sw128(smem_addr(smem), 16, 1024);
+    for (int kb = kb0; ok && kb < kb1; kb += KSUB) {
+      ok = __all_sync(0xffffffffu, fp8::wait(&full[s], phase, ctx, kErrMmaFull));
+      if (!ok) break;
+#pragma unroll
+      for (int sub = 0; sub < KSUB; ++sub) {
+        if (kb + sub >= kb1) break;
+        ok = __all_sync(0xffffffffu, fp8::wait(&tmem_empty[buf], buf_phase, ctx, kErrMmaTmemEmpty));
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (one) {
+          const uint64_t b = desc0 + ((s * L::kStageBytes + sub * L::kSub) >> 4);
+          const uint64_t a = b + (L::kBBytes >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / fp8::kMmaK; ++kk) {
+            const uint64_t step = kk * fp8::kMmaK >> 4;
+            fp8::mma(tmem_base + buf * L::kMmaN, (kSwap ? b : a) + step, (kSwap ? a : b) + step, p.idesc, kk != 0 ? 1u : 0u);
+          }
+          umma_commit(&tmem_full[buf]);
+          if (sub == KSUB - 1) umma_commit(&empty[s]);
+        }
+        __syncwarp();
+        issued = true;
+        if (++buf == kBufs) buf = 0, buf_phase ^= 1u;
+      }
+      if (++s == STAGES) s = 0, phase ^= 1u;
+    }
+    if (!ok && issued && one) {
+      umma_commit(drain);
+      mbar_wait_quiet(drain, 0, 200000000ull);
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // Scales: warp 2 + q serves the blocks of parity q. Slot i % 8 is rewritten once phase i - 4 of its
+    // buffer is complete: its MMAs were issued after every warp had read block i - 8.
+    bool ok = true;
+    for (int kb = kb0 + warp - 2; ok && kb < kb1; kb += 2) {
+      const uint32_t i = static_cast<uint32_t>(kb - kb0), buf = i % kBufs;
+      const float* sa = p.a_scale + kb * p.a_scale_blk;
+      const float* sb = p.b_scale + kb * p.b_scale_blk;
+      constexpr int kA = (TM + 31) / 32;
+      float a[kA], b[kRows ? kBlockN / 32 : 1];
+#pragma unroll
+      for (int j = 0; j < kA; ++j) {
+        const int r = j * 32 + lane;
+        a[j] = r < TM && m0 + r < p.m ? __ldg(sa + (m0 + r) * p.a_scale_row) : 0.0f;
+      }
+      if constexpr (kRows) {
+#pragma unroll
+        for (int j = 0; j < kBlockN / 32; ++j) {
+          const int r = n0 + j * 32 + lane;
+          b[j] = r < p.n ? __ldg(sb + r * p.b_scale_row) : 0.0f;
+        }
+      } else {
+        b[0] = __ldg(sb + (n0 / kBlockN) * p.b_scale_row);
+      }
+      if (i >= kBufs) ok = fp8::wait(&tmem_full[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrScaleTmemFull);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      float* slot = slots + (i % kSlots) * L::kSlotFloats;
+#pragma unroll
+      for (int j = 0; j < kA; ++j)
+        if (j * 32 + lane < TM) slot[j * 32 + lane] = kRows ? a[j] : a[j] * b[0];
+      if constexpr (kRows) {
+#pragma unroll
+        for (int j = 0; j < kBlockN / 32; ++j) slot[TM + j * 32 + lane] = b[j];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tmem_full[buf]);
+    }
+  } else {
+    // ------------------------------------------------------------ accumulation
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;  // TMEM lane
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    constexpr bool kFragments = kRows && !kSwap;
+    constexpr int kSteps = L::kMmaN / 16;
+    float acc[L::kMmaN];
+#pragma unroll
+    for (int j = 0; j < L::kMmaN; ++j) acc[j] = 0.0f;
+    bool ok = true;
+    uint32_t buf = 0, phase = 0;
+#pragma unroll 1
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const float* slot = slots + ((kb - kb0) % kSlots) * L::kSlotFloats;
+      ok = __all_sync(0xffffffffu, fp8::wait(&tmem_full[buf], phase, ctx, kErrAccTmemFull));
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint32_t t0 = taddr + buf * L::kMmaN;
+      uint32_t v[2][16];
+      auto load = [&](int c, uint32_t(&r)[16]) {
+        if constexpr (kFragments) fp8::tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>(c & 1) * 16) << 16) + (c >> 1) * 32, r);
+        else fp8::tmem_ld_x16(t0 + c * 16, r);
+      };
+      load(0, v[0]);
+      const float mine = kSwap ? (kRows ? slot[TM + row] : 1.0f) : (kFragments ? 1.0f : slot[row]);
+      float lo_hi[4];
+      if constexpr (kFragments) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lo_hi[j] = slot[quarter * 32 + j * 8 + (lane >> 2)];
+      }
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        uint32_t(&r)[16] = v[c & 1];
+        fp8::tmem_ld_wait_x16(r);
+        if (c + 1 < kSteps) {
+          load(c + 1, v[(c + 1) & 1]);
+        } else {
+          tc_fence_before_sync();
+          if constexpr (!kSwap && !kFragments) {  // nothing of the slot is read after this
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tmem_empty[buf]);
+          }
+        }
+        if constexpr (kFragments) {
+          const float2* sb = reinterpret_cast<const float2*>(slot + TM) + (lane & 3);
+          const float lo = lo_hi[2 * (c & 1)], hi = lo_hi[2 * (c & 1) + 1];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float2 s = sb[((c >> 1) * 4 + g) * 4];
+            float* q = acc + (c >> 1) * 32 + (c & 1) * 16 + 4 * g;
+            q[0] = fmaf(s.x * lo, __uint_as_float(r[4 * g]), q[0]);
+            q[1] = fmaf(s.y * lo, __uint_as_float(r[4 * g + 1]), q[1]);
+            q[2] = fmaf(s.x * hi, __uint_as_float(r[4 * g + 2]), q[2]);
+            q[3] = fmaf(s.y * hi, __uint_as_float(r[4 * g + 3]), q[3]);
+          }
+        } else if constexpr (kSwap) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(slot + c * 16 + j);
+            const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              acc[c * 16 + j + q] = fmaf(kRows ? f[q] * mine : f[q], __uint_as_float(r[j + q]), acc[c * 16 + j + q]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(mine, __uint_as_float(r[j]), acc[c * 16 + j]);
+        }
+      }
+      if constexpr (kSwap || kFragments) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tmem_empty[buf]);
+      }
+      if (++buf == kBufs) buf = 0, phase ^= 1u;
+    }
+    if (ok) {  // the partial tile: every load has landed and every MMA has read it
+      if constexpr (kSwap) {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) red[j * kBlockN + row] = acc[j];
+      } else if constexpr (kFragments) {
+#pragma unroll
+        for (int j = 0; j < kBlockN; j += 2) {
+          const int m = quarter * 32 + 16 * ((j >> 4) & 1) + 8 * ((j >> 1) & 1) + (lane >> 2);
+          const int g = 8 * (j >> 5) + 2 * ((j >> 2) & 3) + ((lane & 3) >> 1);
+          *reinterpret_cast<float2*>(red + red_at<kSwap>(m, g) + 2 * (lane & 1)) = make_float2(acc[j], acc[j + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < kBlockN / 4; ++g)
+          *reinterpret_cast<float4*>(red + red_at<kSwap>(row, g)) =
+              make_float4(acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]);
+      }
+    }
+  }
+
+  // Every thread of every CTA of the cluster reaches both barriers, also on the abort path.
+  tc_fence_before_sync();
+  __syncwarp();
+  if (p.splits > 1) cluster_sync_all();
+  else __syncthreads();
+  {
+    const uint32_t red_addr = smem_addr(red);
+    constexpr int kGroups = kBlockN / 4;  // 4 consecutive n
+    const int g0 = split * kGroups / p.splits, groups = (split + 1) * kGroups / p.splits - g0;
+    const int rows = p.m - m0 < TM ? p.m - m0 : TM;
+    const int total = groups * rows;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+      const int mi = i / groups, g = g0 + i % groups;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (p.splits == 1) {
+        const float4 f = *reinterpret_cast<const float4*>(red + red_at<kSwap>(mi, g));
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+      } else {
+        const uint32_t off = static_cast<uint32_t>(red_at<kSwap>(mi, g) * 4);
+        float4 part[kMaxSplits];
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+          if (s < p.splits) part[s] = fp8::ld_dsmem_v4f(red_addr + off, static_cast<uint32_t>(s));
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+          if (s < p.splits) v[0] += part[s].x, v[1] += part[s].y, v[2] += part[s].z, v[3] += part[s].w;
+      }
+      const int n = n0 + 4 * g;
+      const int64_t at = static_cast<int64_t>(m0 + mi) * p.ldd + n;
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.n) v[j] += fp8::load_out(p.bias, n + j, p.d_type);
+      }
+      if (p.vec_d && n + 4 <= p.n) {
+        if (p.d_type == fp8::kF32)
+          *reinterpret_cast<float4*>(static_cast<float*>(p.d) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.d) + at) =
+              make_uint2(fp8::pack_out(v[0], v[1], p.d_type), fp8::pack_out(v[2], v[3], p.d_type));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.n) fp8::store_out(p.d, at + j, p.d_type, v[j]);
+      }
+    }
+  }
+  __syncwarp();
+  if (p.splits > 1) cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, L::kTmemCols);
+  }
+}
+
+}  // namespace fp8_tile
+}  // namespace zcb

@@ -12,7 +12,7 @@
 #include "kernels/quantize_fp8.cuh"
 #include "kernels/rotary.cuh"
 #include "kernels/sm100_fp8_pair.cuh"
-#include "kernels/sm100_fp8_swapab.cuh"
+#include "kernels/sm100_fp8_tile.cuh"
 #include "launchers.hpp"
 #include "tma_desc.hpp"
 
@@ -122,14 +122,13 @@ struct Fp8Types {
   int d_bytes() const { return d == ZCUTLASS_F32 ? 4 : 2; }
 };
 
-template <int MP, int STAGES, int KSUB>
-cudaError_t swap_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, int splits, cudaStream_t stream) {
-  using L = fp8_swap::Smem<MP, STAGES, KSUB>;
-  CUtensorMap tw, tx;
-  if (!fp8_map(&tw, g.b, g.n, g.k, g.ldb, fp8_swap::kBlockN) || !fp8_map(&tx, g.a, g.m, g.k, g.lda, MP))
+template <bool kSwap, int TM, int STAGES, int KSUB>
+cudaError_t tile_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, int splits, cudaStream_t stream) {
+  CUtensorMap ta, tb;
+  if (!fp8_map(&ta, g.a, g.m, g.k, g.lda, TM) || !fp8_map(&tb, g.b, g.n, g.k, g.ldb, fp8_tile::kBlockN))
     return cudaErrorInvalidValue;
-  const int64_t tiles_m = div_up(g.m, MP);
-  Fp8SwapParams p{};
+  const int64_t tiles_m = div_up(g.m, TM);
+  Fp8TileParams p{};
   p.m = static_cast<int>(g.m), p.n = static_cast<int>(g.n);
   p.num_kb = static_cast<int>(div_up(g.k, fp8::kBlockK));
   p.splits = splits;
@@ -139,15 +138,17 @@ cudaError_t swap_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo
   p.d = g.d, p.ldd = g.ldd, p.d_type = t.d;
   p.vec_d = g.ldd % 4 == 0 && aligned(g.d, 4 * t.d_bytes());
   p.bias = g.bias;
-  p.idesc = fp8::idesc(fp8_swap::kBlockN, MP, t.b5, t.a5);
+  p.idesc = kSwap ? fp8::idesc(fp8_tile::kBlockN, TM, t.b5, t.a5) : fp8::idesc(TM, fp8_tile::kBlockN, t.a5, t.b5);
   p.error_word = dev.error_word;
-  const int64_t grid = tiles_m * div_up(g.n, fp8_swap::kBlockN) * splits;
+  const int64_t grid = tiles_m * div_up(g.n, fp8_tile::kBlockN) * splits;
   static std::atomic<uint64_t> ready[2];
   if (g.b_scale_rows == 1)
-    return launch_cluster(fp8_swap::gemm_kernel<MP, STAGES, KSUB, true>, ready[1], dev, L::kDynamicBytes, grid,
-                          fp8_swap::kThreads, splits, stream, tw, tx, p);
-  return launch_cluster(fp8_swap::gemm_kernel<MP, STAGES, KSUB, false>, ready[0], dev, L::kDynamicBytes, grid,
-                        fp8_swap::kThreads, splits, stream, tw, tx, p);
+    return launch_cluster(fp8_tile::gemm_kernel<kSwap, TM, true, STAGES, KSUB>, ready[1], dev,
+                          fp8_tile::Smem<kSwap, TM, true, STAGES, KSUB>::kDynamicBytes, grid, fp8_tile::kThreads, splits,
+                          stream, ta, tb, p);
+  return launch_cluster(fp8_tile::gemm_kernel<kSwap, TM, false, STAGES, KSUB>, ready[0], dev,
+                        fp8_tile::Smem<kSwap, TM, false, STAGES, KSUB>::kDynamicBytes, grid, fp8_tile::kThreads, splits,
+                        stream, ta, tb, p);
 }
 
 cudaError_t pair_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, cudaStream_t stream) {
@@ -183,7 +184,7 @@ cudaError_t pair_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo
                         ta, tb, td, p);
 }
 
-// ZCUTLASS_FORCE_KERNEL=fp8_generic | fp8_swap<rows> | fp8_pair pins the kernel of the 8-bit product
+// ZCUTLASS_FORCE_KERNEL=fp8_generic | fp8_tile<rows> | fp8_pair pins the kernel of the 8-bit product
 // (tests); other values concern the 16-bit GEMM alone.
 bool forced(const char* kernel) {
   const char* f = std::getenv("ZCUTLASS_FORCE_KERNEL");
@@ -194,23 +195,24 @@ bool any_forced() {
   return f != nullptr && std::strncmp(f, "fp8_", 4) == 0;
 }
 
-// CTAs along K per tile of the swapped kernel: as many as fit the SMs' slots at once, each with at least
-// two blocks, at most a cluster of 8.
-int swap_splits(int64_t tiles, int64_t num_kb, int64_t slots) {
+// CTAs along K per tile: as many as fit the SMs' slots at once, each with at least two blocks, at most a
+// cluster of 8.
+int tile_splits(int64_t tiles, int64_t num_kb, int64_t slots) {
   const char* v = std::getenv("ZCUTLASS_SPLITK");
   int64_t s = v != nullptr && v[0] != '\0' ? std::atoi(v) : slots / std::max<int64_t>(tiles, 1);
-  s = std::min<int64_t>(s, std::min<int64_t>(fp8_swap::kMaxSplits, num_kb / 2));
+  s = std::min<int64_t>(s, std::min<int64_t>(fp8_tile::kMaxSplits, num_kb / 2));
   return static_cast<int>(std::max<int64_t>(s, 1));
 }
 
 cudaError_t tensor_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, cudaStream_t stream) {
   const int64_t tiles_n = div_up(g.n, 128), kb = div_up(g.k, fp8::kBlockK), sms = dev.sm_count;
   const bool any = any_forced();
+  const auto splits = [&](int tm, int64_t slots) { return tile_splits(tiles_n * div_up(g.m, tm), kb, slots); };
   if (any ? forced("fp8_pair") : div_up(g.m, 256) * div_up(g.n, 256) >= sms / 4) return pair_fp8(g, t, dev, stream);
-  if (any ? forced("fp8_swap16") : g.m <= 16) return swap_fp8<16, 3, 2>(g, t, dev, swap_splits(tiles_n * div_up(g.m, 16), kb, 2 * sms), stream);
-  if (any ? forced("fp8_swap32") : g.m <= 32) return swap_fp8<32, 5, 1>(g, t, dev, swap_splits(tiles_n * div_up(g.m, 32), kb, 2 * sms), stream);
-  if (any ? forced("fp8_swap64") : g.m <= 64) return swap_fp8<64, 4, 1>(g, t, dev, swap_splits(tiles_n * div_up(g.m, 64), kb, 2 * sms), stream);
-  return swap_fp8<128, 3, 2>(g, t, dev, swap_splits(tiles_n * div_up(g.m, 128), kb, sms), stream);
+  if (any ? forced("fp8_tile16") : g.m <= 16) return tile_fp8<true, 16, 3, 2>(g, t, dev, splits(16, 2 * sms), stream);
+  if (any ? forced("fp8_tile32") : g.m <= 32) return tile_fp8<true, 32, 5, 1>(g, t, dev, splits(32, 2 * sms), stream);
+  if (any ? forced("fp8_tile64") : g.m <= 64) return tile_fp8<true, 64, 4, 1>(g, t, dev, splits(64, 2 * sms), stream);
+  return tile_fp8<false, 128, 3, 2>(g, t, dev, splits(128, sms), stream);
 }
 
 template <typename T, int V>
