@@ -166,34 +166,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
       // ------------------------------------------------------------ producer (both CTAs)
-      if (lane == 0) {
-        uint32_t it = 0;
-        bool ok = true;
-        for (int tile = pair; ok && tile < p.total_tiles; tile += npairs) {
-          int tm, tn;
-          raster(tile, p, tm, tn);
-          const int m0 = tm * kBlock + static_cast<int>(rank) * kHalf;
-          const int n0 = tn * kBlock + static_cast<int>(rank) * kHalf;
-          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-            const uint32_t s = it % kStages;
-            if (!fp8::wait(&empty[s], ((it / kStages) & 1u) ^ 1u, ctx, kErrProducerEmpty)) {
-              ok = false;
-              break;
-            }
+      const bool one = fp8::elect_one();
+      uint32_t s = 0, phase = 1, it = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < p.total_tiles; tile += npairs) {
+        int tm, tn;
+        raster(tile, p, tm, tn);
+        const int m0 = tm * kBlock + static_cast<int>(rank) * kHalf;
+        const int n0 = tn * kBlock + static_cast<int>(rank) * kHalf;
+        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+          ok = __all_sync(0xffffffffu, fp8::wait(&empty[s], phase, ctx, kErrProducerEmpty));
+          if (!ok) break;
+          if (one) {
             const uint32_t full_leader = map_shared_rank(smem_addr(&full[s]), 0);
             if (leader) mbar_arrive_expect_tx(&full[s], 2 * L::kStageBytes);
             uint8_t* at = smem + s * L::kStageBytes;
             tma_load_2d_pair(at, &tmap_a, full_leader, kb * kBlockK, m0);
             tma_load_2d_pair(at + L::kOperand, &tmap_b, full_leader, kb * kBlockK, n0);
           }
+          __syncwarp();
+          if (++s == kStages) s = 0, phase ^= 1u;
         }
-        if (!ok) {  // unwind: loads already issued must land before the CTAs can exit
-          if (leader) {
-            const uint32_t first = it > static_cast<uint32_t>(kStages) ? it - kStages : 0u;
-            for (uint32_t j = first; j < it; ++j) mbar_wait_quiet(&full[j % kStages], (j / kStages) & 1u, 200000000ull);
-          } else {
-            for (int i = 0; i < 1000; ++i) sleep_ns(1000);  // the follower cannot poll the leader's barrier
-          }
+      }
+      if (!ok && one) {  // unwind: loads already issued must land before the CTAs can exit
+        if (leader) {
+          const uint32_t first = it > static_cast<uint32_t>(kStages) ? it - kStages : 0u;
+          for (uint32_t j = first; j < it; ++j) mbar_wait_quiet(&full[j % kStages], (j / kStages) & 1u, 200000000ull);
+        } else {
+          for (int i = 0; i < 1000; ++i) sleep_ns(1000);  // the follower cannot poll the leader's barrier
         }
       }
       __syncwarp();

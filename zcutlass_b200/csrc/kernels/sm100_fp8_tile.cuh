@@ -140,32 +140,33 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
   const WaitCtx ctx{abort_flag, p.error_word};
 
   if (warp == 0) {
-    if (lane == 0) {
-      // B is read once when one tile of rows covers M; A by every CTA.
-      const uint64_t b_policy = p.tiles_m == 1 ? l2_policy_evict_first() : l2_policy_evict_last();
-      const uint64_t a_policy = l2_policy_evict_last();
-      uint32_t it = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; kb += KSUB, ++it) {
-        const uint32_t s = it % STAGES;
-        if (!fp8::wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, ctx, kErrProducerEmpty)) {
-          ok = false;
-          break;
-        }
-        const int subs = kb1 - kb < KSUB ? kb1 - kb : KSUB;
+    // The whole warp walks the loop (uniform registers), one lane issues. B is read once when one tile of
+    // rows covers M; A by every CTA.
+    const bool one = fp8::elect_one();
+    const uint64_t b_policy = p.tiles_m == 1 ? l2_policy_evict_first() : l2_policy_evict_last();
+    const uint64_t a_policy = l2_policy_evict_last();
+    uint32_t s = 0, phase = 1, it = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; kb += KSUB, ++it) {
+      ok = __all_sync(0xffffffffu, fp8::wait(&empty[s], phase, ctx, kErrProducerEmpty));
+      if (!ok) break;
+      const int subs = kb1 - kb < KSUB ? kb1 - kb : KSUB;
+      if (one) {
         mbar_arrive_expect_tx(&full[s], subs * L::kSub);
+        uint8_t* at = smem + s * L::kStageBytes;
 #pragma unroll
         for (int sub = 0; sub < KSUB; ++sub) {
           if (sub >= subs) break;
-          uint8_t* at = smem + s * L::kStageBytes + sub * L::kSub;
-          tma_load_2d_hint(at, &tmap_b, &full[s], (kb + sub) * kBlockK, n0, b_policy);
-          tma_load_2d_hint(at + L::kBBytes, &tmap_a, &full[s], (kb + sub) * kBlockK, m0, a_policy);
+          tma_load_2d_hint(at + sub * L::kSub, &tmap_b, &full[s], (kb + sub) * kBlockK, n0, b_policy);
+          tma_load_2d_hint(at + sub * L::kSub + L::kBBytes, &tmap_a, &full[s], (kb + sub) * kBlockK, m0, a_policy);
         }
       }
-      if (!ok) {  // loads already issued must land before the CTA can exit
-        const uint32_t first = it > static_cast<uint32_t>(STAGES) ? it - STAGES : 0u;
-        for (uint32_t j = first; j < it; ++j) mbar_wait_quiet(&full[j % STAGES], (j / STAGES) & 1u, 200000000ull);
-      }
+      __syncwarp();
+      if (++s == STAGES) s = 0, phase ^= 1u;
+    }
+    if (!ok && one) {  // loads already issued must land before the CTA can exit
+      const uint32_t first = it > static_cast<uint32_t>(STAGES) ? it - STAGES : 0u;
+      for (uint32_t j = first; j < it; ++j) mbar_wait_quiet(&full[j % STAGES], (j / STAGES) & 1u, 200000000ull);
     }
     __syncwarp();
   } else if (warp == 1) {

@@ -195,11 +195,13 @@ bool any_forced() {
   return f != nullptr && std::strncmp(f, "fp8_", 4) == 0;
 }
 
-// CTAs along K per tile: as many as fit the SMs' slots at once, each with at least two blocks, at most a
-// cluster of 8.
-int tile_splits(int64_t tiles, int64_t num_kb, int64_t slots) {
+// CTAs along K per tile, each with at least two blocks, at most a cluster of 8. The swapped kernel, two CTAs
+// of which fit an SM: as few as give (nearly) every SM one, since more only add partial tiles to exchange:
+// 16 x 4096 x 4096 (32 tiles) takes 8.3, 6.5 and 7.6 us with 2, 4 and 8 splits, 1 x 6144 x 4096 (48 tiles)
+// 8.6, 8.4, 8.0 and 12.1 with 2, 3, 4 and 6. The other, one CTA of which fills an SM: as many as run at once.
+int tile_splits(int64_t tiles, int64_t num_kb, int64_t sms, bool swap) {
   const char* v = std::getenv("ZCUTLASS_SPLITK");
-  int64_t s = v != nullptr && v[0] != '\0' ? std::atoi(v) : slots / std::max<int64_t>(tiles, 1);
+  int64_t s = v != nullptr && v[0] != '\0' ? std::atoi(v) : swap ? div_up(sms * 6 / 7, tiles) : sms / tiles;
   s = std::min<int64_t>(s, std::min<int64_t>(fp8_tile::kMaxSplits, num_kb / 2));
   return static_cast<int>(std::max<int64_t>(s, 1));
 }
@@ -207,12 +209,17 @@ int tile_splits(int64_t tiles, int64_t num_kb, int64_t slots) {
 cudaError_t tensor_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, cudaStream_t stream) {
   const int64_t tiles_n = div_up(g.n, 128), kb = div_up(g.k, fp8::kBlockK), sms = dev.sm_count;
   const bool any = any_forced();
-  const auto splits = [&](int tm, int64_t slots) { return tile_splits(tiles_n * div_up(g.m, tm), kb, slots); };
-  if (any ? forced("fp8_pair") : div_up(g.m, 256) * div_up(g.n, 256) >= sms / 4) return pair_fp8(g, t, dev, stream);
-  if (any ? forced("fp8_tile16") : g.m <= 16) return tile_fp8<true, 16, 3, 2>(g, t, dev, splits(16, 2 * sms), stream);
-  if (any ? forced("fp8_tile32") : g.m <= 32) return tile_fp8<true, 32, 5, 1>(g, t, dev, splits(32, 2 * sms), stream);
-  if (any ? forced("fp8_tile64") : g.m <= 64) return tile_fp8<true, 64, 4, 1>(g, t, dev, splits(64, 2 * sms), stream);
-  return tile_fp8<false, 128, 3, 2>(g, t, dev, splits(128, sms), stream);
+  const auto splits = [&](int tm) { return tile_splits(tiles_n * div_up(g.m, tm), kb, sms, tm < 128); };
+  if (any ? forced("fp8_tile16") : g.m <= 16) return tile_fp8<true, 16, 3, 2>(g, t, dev, splits(16), stream);
+  if (any ? forced("fp8_tile32") : g.m <= 32) return tile_fp8<true, 32, 5, 1>(g, t, dev, splits(32), stream);
+  if (any ? forced("fp8_tile64") : g.m <= 64) return tile_fp8<true, 64, 4, 1>(g, t, dev, splits(64), stream);
+  // Above that, whichever takes fewer waves of tiles: a wave takes about as long with 128 x 128 tiles on
+  // every SM as with 256 x 256 tiles on every pair (18.3 and 18.5 us at K = 4096), and one wave of the former
+  // can be shortened by splitting K.
+  const int64_t waves = div_up(tiles_n * div_up(g.m, 128), sms);
+  const int64_t pair_waves = div_up(div_up(g.m, 256) * div_up(g.n, 256), sms / 2);
+  if (any ? forced("fp8_pair") : waves > 1 && pair_waves <= waves) return pair_fp8(g, t, dev, stream);
+  return tile_fp8<false, 128, 3, 2>(g, t, dev, splits(128), stream);
 }
 
 template <typename T, int V>
