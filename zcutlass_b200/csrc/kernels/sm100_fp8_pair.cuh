@@ -344,16 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               tc_fence_before_sync();
             }
-            const float lo = sa[2 * (c & 1)], hi = sa[2 * (c & 1) + 1];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float2 s = sb[((c >> 1) * 4 + g) * 4];
-              float* q = acc + (c >> 1) * 32 + (c & 1) * 16 + 4 * g;
-              q[0] = fmaf(s.x * lo, __uint_as_float(r[4 * g]), q[0]);
-              q[1] = fmaf(s.y * lo, __uint_as_float(r[4 * g + 1]), q[1]);
-              q[2] = fmaf(s.x * hi, __uint_as_float(r[4 * g + 2]), q[2]);
-              q[3] = fmaf(s.y * hi, __uint_as_float(r[4 * g + 3]), q[3]);
-            }
+            fp8::add_fragments(acc + (c >> 1) * 32 + (c & 1) * 16, r, sb + (c >> 1) * 16, sa[2 * (c & 1)], sa[2 * (c & 1) + 1]);
           }
           __syncwarp();  // the slot has been read, too
           if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));

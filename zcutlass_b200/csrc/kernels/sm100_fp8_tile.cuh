@@ -135,6 +135,11 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  // Weights of the first stages on their way to L2 while the kernel before (often the quantisation of A) is
+  // still running. A hint: if that kernel writes them, the copies in L2 are what it writes.
+  if (warp == 0 && lane == 0) {
+    for (int kb = kb0; kb < kb1 && kb < kb0 + STAGES * KSUB; ++kb) fp8::tma_prefetch_2d(&tmap_b, kb * kBlockK, n0);
+  }
   griddep_wait();
   griddep_launch_dependents();
   const WaitCtx ctx{abort_flag, p.error_word};
@@ -289,16 +294,7 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
         }
         if constexpr (kFragments) {
           const float2* sb = reinterpret_cast<const float2*>(slot + TM) + (lane & 3);
-          const float lo = lo_hi[2 * (c & 1)], hi = lo_hi[2 * (c & 1) + 1];
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float2 s = sb[((c >> 1) * 4 + g) * 4];
-            float* q = acc + (c >> 1) * 32 + (c & 1) * 16 + 4 * g;
-            q[0] = fmaf(s.x * lo, __uint_as_float(r[4 * g]), q[0]);
-            q[1] = fmaf(s.y * lo, __uint_as_float(r[4 * g + 1]), q[1]);
-            q[2] = fmaf(s.x * hi, __uint_as_float(r[4 * g + 2]), q[2]);
-            q[3] = fmaf(s.y * hi, __uint_as_float(r[4 * g + 3]), q[3]);
-          }
+          fp8::add_fragments(acc + (c >> 1) * 32 + (c & 1) * 16, r, sb + (c >> 1) * 16, lo_hi[2 * (c & 1)], lo_hi[2 * (c & 1) + 1]);
         } else if constexpr (kSwap) {
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
@@ -345,36 +341,27 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
   if (p.splits > 1) cluster_sync_all();
   else __syncthreads();
   {
+    // CTA r of the cluster adds the partial tiles of its 4-column groups: thread t takes group t % groups of
+    // rows t / groups, t / groups + per, ...
     const uint32_t red_addr = smem_addr(red);
-    constexpr int kGroups = kBlockN / 4;  // 4 consecutive n
+    constexpr int kGroups = kBlockN / 4;
     const int g0 = split * kGroups / p.splits, groups = (split + 1) * kGroups / p.splits - g0;
     const int rows = p.m - m0 < TM ? p.m - m0 : TM;
-    const int total = groups * rows;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-      const int mi = i / groups, g = g0 + i % groups;
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (p.splits == 1) {
-        const float4 f = *reinterpret_cast<const float4*>(red + red_at<kSwap>(mi, g));
-        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-      } else {
-        const uint32_t off = static_cast<uint32_t>(red_at<kSwap>(mi, g) * 4);
-        float4 part[kMaxSplits];
+    const int per = kThreads / groups;
+    const int first = static_cast<int>(threadIdx.x) / groups;
+    const int g = g0 + static_cast<int>(threadIdx.x) % groups;
+    const int n = n0 + 4 * g;
+    float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias != nullptr) {
 #pragma unroll
-        for (int s = 0; s < kMaxSplits; ++s)
-          if (s < p.splits) part[s] = fp8::ld_dsmem_v4f(red_addr + off, static_cast<uint32_t>(s));
-#pragma unroll
-        for (int s = 0; s < kMaxSplits; ++s)
-          if (s < p.splits) v[0] += part[s].x, v[1] += part[s].y, v[2] += part[s].z, v[3] += part[s].w;
-      }
-      const int n = n0 + 4 * g;
+      for (int j = 0; j < 4; ++j)
+        if (n + j < p.n) bias[j] = fp8::load_out(p.bias, n + j, p.d_type);
+    }
+    const bool whole = p.vec_d && n + 4 <= p.n;
+    auto put = [&](int mi, const float4& f) {
+      const float v[4] = {f.x + bias[0], f.y + bias[1], f.z + bias[2], f.w + bias[3]};
       const int64_t at = static_cast<int64_t>(m0 + mi) * p.ldd + n;
-      if (p.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.n) v[j] += fp8::load_out(p.bias, n + j, p.d_type);
-      }
-      if (p.vec_d && n + 4 <= p.n) {
+      if (whole) {
         if (p.d_type == fp8::kF32)
           *reinterpret_cast<float4*>(static_cast<float*>(p.d) + at) = make_float4(v[0], v[1], v[2], v[3]);
         else
@@ -385,10 +372,30 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
         for (int j = 0; j < 4; ++j)
           if (n + j < p.n) fp8::store_out(p.d, at + j, p.d_type, v[j]);
       }
+    };
+    if (p.splits == 1) {
+#pragma unroll 4
+      for (int mi = first; mi < rows; mi += per) put(mi, *reinterpret_cast<const float4*>(red + red_at<kSwap>(mi, g)));
+    } else if (first < per) {
+#pragma unroll 2
+      for (int mi = first; mi < rows; mi += per) {
+        const uint32_t off = static_cast<uint32_t>(red_at<kSwap>(mi, g) * 4);
+        float4 part[kMaxSplits];
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+          if (s < p.splits) part[s] = fp8::ld_dsmem_v4f(red_addr + off, static_cast<uint32_t>(s));
+        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+          if (s < p.splits) f.x += part[s].x, f.y += part[s].y, f.z += part[s].z, f.w += part[s].w;
+        put(mi, f);
+      }
     }
   }
   __syncwarp();
-  if (p.splits > 1) cluster_sync_all();
+  // No CTA leaves while a peer may still read its partial tile. The reads are done (their sums were used) and
+  // nothing is handed over, so the arrival need not wait for the stores to D.
+  if (p.splits > 1) fp8::cluster_sync_relaxed();
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, L::kTmemCols);
