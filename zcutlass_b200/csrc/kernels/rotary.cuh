@@ -32,6 +32,7 @@ struct RotaryParams {
   int64_t table_rows, table_ld;
   int head_dim, rotary_dim;
   bool inverse;
+  bool small;       // thread indices fit 31 bits
   int head_lanes;   // threads that share a token's heads
   int items;        // vector positions per head
   int* error_word;
@@ -42,127 +43,148 @@ namespace rotary {
 constexpr int kThreads = 256;
 constexpr int kErrPosition = (32 << 4) | 1;
 
+// V values of T moved as one access (16 bytes, or one value).
 template <typename T, int V>
-struct Pack;  // V values of T moved as one access
-template <typename T>
-struct Pack<T, 8> {
-  static_assert(sizeof(T) == 2, "");
-  __device__ static void load(const T* p, float (&v)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Elem<T>::unpack(w[i]);
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+struct Pack {
+  static_assert(V == 1 || V * sizeof(T) == 16, "");
+  static constexpr int kWords = V == 1 ? 1 : 4;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 1) {
+      if constexpr (sizeof(T) == 4) w[0] = __float_as_uint(*p);
+      else w[0] = __float_as_uint(Elem<T>::to_float(*p));
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
     }
   }
-  __device__ static void store(T* p, const float (&v)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]),
-                                              Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (V == 1) {
+      if constexpr (sizeof(T) == 4) *p = __uint_as_float(w[0]);
+      else *p = Elem<T>::from_float(__uint_as_float(w[0]));
+    } else {
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
-};
-template <>
-struct Pack<float, 4> {
-  __device__ static void load(const float* p, float (&v)[4]) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+    if constexpr (V == 1 || sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const float2 f = Elem<T>::unpack(w[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      }
+    }
   }
-  __device__ static void store(float* p, const float (&v)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-};
-template <typename T>
-struct Pack<T, 1> {
-  __device__ static void load(const T* p, float (&v)[1]) {
-    if constexpr (sizeof(T) == 4) v[0] = *p;
-    else v[0] = Elem<T>::to_float(*p);
-  }
-  __device__ static void store(T* p, const float (&v)[1]) {
-    if constexpr (sizeof(T) == 4) *p = v[0];
-    else *p = Elem<T>::from_float(v[0]);
+  __device__ __forceinline__ void set(const float (&v)[V]) {
+    if constexpr (V == 1 || sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) w[i] = Elem<T>::pack(v[2 * i], v[2 * i + 1]);
+    }
   }
 };
 
 // Vector positions of a head: half layout, V pairs per item (two accesses of V values), then
 // (head_dim - rotary_dim) / V items that pass through; interleaved layout, V / 2 pairs in one access
 // (V = 1: the two values of a pair), then the same. V = 1 takes any stride, alignment and size.
+// A thread takes kBatch heads at a time, all their loads before the first store (in place, the compiler may
+// not move a load over a store).
 template <typename T, int V, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  const int per_token = p.items * p.head_lanes;
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t token = idx / per_token;
-  if (token >= p.tokens) return;
-  const int rest = static_cast<int>(idx - token * per_token);
-  const int item = rest % p.items;
-  const int half = p.rotary_dim / 2;
-  constexpr int kStep = kInterleaved ? (V == 1 ? 2 : V) : V;  // values per access step of one item
+  constexpr int kBatch = 4;
+  constexpr int kParts = kInterleaved && V > 1 ? 1 : 2;      // accesses per item
   constexpr int kPairs = kInterleaved ? (V == 1 ? 1 : V / 2) : V;
+  const uint32_t per_token = static_cast<uint32_t>(p.items) * p.head_lanes;
+  int64_t token;
+  uint32_t rest;
+  if (p.small) {  // 32-bit division
+    const uint32_t idx = blockIdx.x * kThreads + threadIdx.x;
+    const uint32_t t = idx / per_token;
+    token = t, rest = idx - t * per_token;
+  } else {
+    const int64_t idx = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    token = idx / per_token, rest = static_cast<uint32_t>(idx - token * per_token);
+  }
+  if (token >= p.tokens) return;
+  const int lane = static_cast<int>(rest / p.items);
+  const int item = static_cast<int>(rest) - lane * p.items;
+  const int half = p.rotary_dim / 2;
   const int rot_items = half / kPairs;
-  const bool turn = item < rot_items;
   const int64_t pos = p.positions64 ? static_cast<const int64_t*>(p.positions)[token]
                                     : static_cast<int64_t>(static_cast<const int32_t*>(p.positions)[token]);
   const bool known = pos >= 0 && pos < p.table_rows;  // below 0: padding; above: an error
   if (pos >= p.table_rows && rest == 0 && p.error_word != nullptr) atomicCAS(p.error_word, 0, kErrPosition);
-  float c[kPairs] = {}, s[kPairs] = {};  // a position outside the table leaves the heads as they are
-  if (turn && known) {
+  const bool rotated = item < rot_items;
+  const bool turn = rotated && known;  // else the values are copied as they are
+  // Offsets of the item's accesses in a head.
+  const int at0 = !rotated ? p.rotary_dim + (item - rot_items) * V : kInterleaved ? (V == 1 ? 2 * item : V * item) : V * item;
+  const int at1 = kInterleaved ? at0 + 1 : at0 + half;
+  const int parts = rotated ? kParts : 1;
+  float c[kPairs] = {}, s[kPairs] = {};
+  if (turn) {
     const float* row = p.table + pos * p.table_ld + item * kPairs;
     if constexpr (kPairs % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < kPairs; i += 4) {
-        const float4 a = *reinterpret_cast<const float4*>(row + i);
-        const float4 b = *reinterpret_cast<const float4*>(row + half + i);
+        const float4 a = __ldg(reinterpret_cast<const float4*>(row + i));
+        const float4 b = __ldg(reinterpret_cast<const float4*>(row + half + i));
         c[i] = a.x, c[i + 1] = a.y, c[i + 2] = a.z, c[i + 3] = a.w;
         s[i] = b.x, s[i + 1] = b.y, s[i + 2] = b.z, s[i + 3] = b.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) c[i] = row[i], s[i] = row[half + i];
+      for (int i = 0; i < kPairs; ++i) c[i] = __ldg(row + i), s[i] = __ldg(row + half + i);
     }
     if (p.inverse) {
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) s[i] = -s[i];
     }
   }
-  const int lane = rest / p.items;
   const int heads = p.x[0].heads + p.x[1].heads;
-#pragma unroll 4
-  for (int h = lane; h < heads; h += p.head_lanes) {
-    const bool second = h >= p.x[0].heads;
-    const RotaryTensor& x = p.x[second ? 1 : 0];
-    const int hh = second ? h - p.x[0].heads : h;
-    const T* in = static_cast<const T*>(x.in) + token * x.in_token + hh * x.in_head;
-    T* out = static_cast<T*>(x.out) + token * x.out_token + hh * x.out_head;
-    if (!turn) {
-      if (in == out) continue;  // in place: nothing to move
-      const int at = p.rotary_dim + (item - rot_items) * V;
-      float v[V];
-      Pack<T, V>::load(in + at, v);
-      Pack<T, V>::store(out + at, v);
-    } else if constexpr (kInterleaved && V > 1) {
-      const int at = item * kStep;
-      float v[V], y[V];
-      Pack<T, V>::load(in + at, v);
+  const T* in0 = static_cast<const T*>(p.x[0].in) + token * p.x[0].in_token;
+  const T* in1 = static_cast<const T*>(p.x[1].in) + token * p.x[1].in_token;
+  T* out0 = static_cast<T*>(p.x[0].out) + token * p.x[0].out_token;
+  T* out1 = static_cast<T*>(p.x[1].out) + token * p.x[1].out_token;
+  for (int h0 = lane; h0 < heads; h0 += kBatch * p.head_lanes) {
+    Pack<T, V> v[kBatch][kParts];
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        y[2 * i] = known ? v[2 * i] * c[i] - v[2 * i + 1] * s[i] : v[2 * i];
-        y[2 * i + 1] = known ? v[2 * i + 1] * c[i] + v[2 * i] * s[i] : v[2 * i + 1];
-      }
-      Pack<T, V>::store(out + at, y);
-    } else {
-      const int a1 = kInterleaved ? 2 * item : item * V;
-      const int a2 = kInterleaved ? 2 * item + 1 : half + item * V;
-      float v1[V], v2[V], y1[V], y2[V];
-      Pack<T, V>::load(in + a1, v1);
-      Pack<T, V>::load(in + a2, v2);
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = h0 + b * p.head_lanes;
+      if (h >= heads) break;
+      const T* in = h < p.x[0].heads ? in0 + h * p.x[0].in_head : in1 + (h - p.x[0].heads) * p.x[1].in_head;
+      v[b][0].load(in + at0);
+      if (kParts == 2 && parts == 2) v[b][kParts - 1].load(in + at1);
+    }
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        y1[i] = known ? v1[i] * c[i] - v2[i] * s[i] : v1[i];
-        y2[i] = known ? v2[i] * c[i] + v1[i] * s[i] : v2[i];
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = h0 + b * p.head_lanes;
+      if (h >= heads) break;
+      T* out = h < p.x[0].heads ? out0 + h * p.x[0].out_head : out1 + (h - p.x[0].heads) * p.x[1].out_head;
+      if (turn) {
+        float x[kParts][V], y[kParts][V];
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) v[b][q].get(x[q]);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          const float x1 = kParts == 1 ? x[0][2 * i] : x[0][i];
+          const float x2 = kParts == 1 ? x[0][(2 * i + 1) % V] : x[kParts - 1][i];
+          const float y1 = x1 * c[i] - x2 * s[i], y2 = x2 * c[i] + x1 * s[i];
+          if constexpr (kParts == 1) y[0][2 * i] = y1, y[0][(2 * i + 1) % V] = y2;
+          else y[0][i] = y1, y[kParts - 1][i] = y2;
+        }
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) v[b][q].set(y[q]);
       }
-      Pack<T, V>::store(out + a1, y1);
-      Pack<T, V>::store(out + a2, y2);
+      v[b][0].store(out + at0);
+      if (kParts == 2 && parts == 2) v[b][kParts - 1].store(out + at1);
     }
   }
 }

@@ -196,12 +196,16 @@ bool any_forced() {
 }
 
 // CTAs along K per tile, each with at least two blocks, at most a cluster of 8. The swapped kernel, two CTAs
-// of which fit an SM: as few as give (nearly) every SM one, since more only add partial tiles to exchange:
-// 16 x 4096 x 4096 (32 tiles) takes 8.3, 6.5 and 7.6 us with 2, 4 and 8 splits, 1 x 6144 x 4096 (48 tiles)
-// 8.6, 8.4, 8.0 and 12.1 with 2, 3, 4 and 6. The other, one CTA of which fills an SM: as many as run at once.
+// of which fit an SM: the power of two that gives (nearly) every SM one, since more only add partial tiles to
+// exchange, and clusters of other sizes leave SMs out: 16 x 4096 x 4096 (32 tiles) takes 8.3, 6.5 and 7.6 us
+// with 2, 4 and 8 splits, 1 x 6144 x 4096 (48 tiles) 8.6, 8.4, 7.4, 8.5 and 12.1 with 2, 3, 4, 5 and 6. The
+// other, one CTA of which fills an SM: as many as run at once.
 int tile_splits(int64_t tiles, int64_t num_kb, int64_t sms, bool swap) {
   const char* v = std::getenv("ZCUTLASS_SPLITK");
-  int64_t s = v != nullptr && v[0] != '\0' ? std::atoi(v) : swap ? div_up(sms * 6 / 7, tiles) : sms / tiles;
+  int64_t s = sms / tiles;
+  if (swap)
+    for (s = 1; s < fp8_tile::kMaxSplits && s * tiles < sms * 6 / 7; s *= 2) {}
+  if (v != nullptr && v[0] != '\0') s = std::atoi(v);
   s = std::min<int64_t>(s, std::min<int64_t>(fp8_tile::kMaxSplits, num_kb / 2));
   return static_cast<int>(std::max<int64_t>(s, 1));
 }
@@ -210,9 +214,19 @@ cudaError_t tensor_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceIn
   const int64_t tiles_n = div_up(g.n, 128), kb = div_up(g.k, fp8::kBlockK), sms = dev.sm_count;
   const bool any = any_forced();
   const auto splits = [&](int tm) { return tile_splits(tiles_n * div_up(g.m, tm), kb, sms, tm < 128); };
+  // Where there is no more than a CTA per SM, one with two blocks per stage and the SM's whole shared memory
+  // streams faster than one made for two per SM (48 x 4096 x 14336: 15.6 against 17.1 us; with 224 CTAs,
+  // 64 x 28672 x 4096, 30.8 against 23.2). 16 rows are served by the same ring both ways.
+  const auto alone = [&](int s) { return tiles_n * s <= sms * 7 / 8; };
   if (any ? forced("fp8_tile16") : g.m <= 16) return tile_fp8<true, 16, 3, 2>(g, t, dev, splits(16), stream);
-  if (any ? forced("fp8_tile32") : g.m <= 32) return tile_fp8<true, 32, 5, 1>(g, t, dev, splits(32), stream);
-  if (any ? forced("fp8_tile64") : g.m <= 64) return tile_fp8<true, 64, 4, 1>(g, t, dev, splits(64), stream);
+  if (any ? forced("fp8_tile32") : g.m <= 32) {
+    const int s = splits(32);
+    return alone(s) ? tile_fp8<true, 32, 4, 2>(g, t, dev, s, stream) : tile_fp8<true, 32, 5, 1>(g, t, dev, s, stream);
+  }
+  if (any ? forced("fp8_tile64") : g.m <= 64) {
+    const int s = splits(64);
+    return alone(s) ? tile_fp8<true, 64, 4, 2>(g, t, dev, s, stream) : tile_fp8<true, 64, 4, 1>(g, t, dev, s, stream);
+  }
   // Above that, whichever takes fewer waves of tiles: a wave takes about as long with 128 x 128 tiles on
   // every SM as with 256 x 256 tiles on every pair (18.3 and 18.5 us at K = 4096), and one wave of the former
   // can be shortened by splitting K.
@@ -229,12 +243,13 @@ cudaError_t rotary_v(RotaryParams p, bool interleaved, cudaStream_t stream, int 
   p.items = p.rotary_dim / 2 / per_item + (p.head_dim - p.rotary_dim) / V;
   const int heads = p.x[0].heads + p.x[1].heads;
   // Threads per token: one per item and head lane. A thread that walks over several heads reuses its
-  // cosines and sines and keeps more loads in flight; but first every SM gets two blocks.
+  // cosines and sines and keeps more loads in flight; but first every SM gets four blocks.
   p.head_lanes = heads;
-  while (p.head_lanes > 1 && (heads + p.head_lanes - 1) / p.head_lanes < 5 &&
-         p.tokens * p.items * p.head_lanes > 4ll * sms * kThreads)
+  while (p.head_lanes > 1 && div_up(heads, p.head_lanes) < 4 && p.tokens * p.items * p.head_lanes > 8ll * sms * kThreads)
     p.head_lanes = (p.head_lanes + 1) / 2;
-  const int64_t blocks = div_up(p.tokens * p.items * p.head_lanes, kThreads);
+  const int64_t threads = p.tokens * p.items * p.head_lanes;
+  p.small = threads < INT_MAX - kThreads;
+  const int64_t blocks = div_up(threads, kThreads);
   return interleaved ? launch(rotary_kernel<T, V, true>, blocks, kThreads, stream, p)
                      : launch(rotary_kernel<T, V, false>, blocks, kThreads, stream, p);
 }
