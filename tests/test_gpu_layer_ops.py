@@ -520,3 +520,70 @@ def test_refusals(cuda_device):
             call()
             pytest.fail(f"call {i} was not refused")
     torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------- decoder layer
+
+
+def layer_by_hand(layer, x, positions, table, interleaved):
+    """The layer's chain, call by call."""
+    s = layer.shape
+    w = lambda linear: (linear.weight.q, linear.weight.scale)  # noqa: E731
+    qkv = torch_ops.linear_fp8(x, *w(layer.qkv), layer.qkv.bias)
+    q, k, _ = qkv.split([s.q_heads * s.head_dim, s.kv_heads * s.head_dim, s.kv_heads * s.head_dim], dim=1)
+    q, k = torch_ops.rotary(q.unflatten(1, (-1, s.head_dim)), k.unflatten(1, (-1, s.head_dim)), positions, table, interleaved)
+    o = torch_ops.linear_fp8(q.flatten(1), *w(layer.o_proj))
+    gate_up = torch_ops.linear_fp8(o, *w(layer.gate_up))
+    return torch_ops.linear_fp8(gate_up[:, : s.intermediate], *w(layer.down))
+
+
+@pytest.mark.parametrize("tokens", [1, 24, 300])
+@pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
+def test_decoder_layer(cuda_device, tokens, interleaved):
+    """8-bit linears and rotary positions in the tensor-parallel decoder layer: eagerly, over two streams
+    and replayed from a graph, the same bits as the calls one by one."""
+    from zcutlass_b200 import tp
+
+    layer = tp.TPDecoderLinears(tp.LayerShape(512, 1280, 8, 2, 64), tp.TPGroup(), cuda_device, BF16, qkv_bias=True)
+    x, positions = rand(tokens, 512, seed=1, dtype=BF16), torch.randint(0, 400, (tokens,), device="cuda")
+    plain = layer.forward(x).clone()
+    table = torch_ops.rotary_table(400, 48, device="cuda")
+    layer.quantize_fp8()
+    layer.quantize_fp8()
+    eight = layer.forward(x).clone()
+    assert not torch.equal(plain, eight)
+    # four chained products of 8-bit factors: each factor off by at most 2^-4 of its value, errors of random
+    # sign; the norm of the difference stays well below the norm of the result
+    assert (eight.double() - plain.double()).norm() < 0.25 * plain.double().norm()
+    layer.enable_rotary(table, interleaved)
+    want = layer_by_hand(layer, x, positions, table, interleaved)
+    assert torch.equal(layer.forward(x, positions=positions), want)
+    if tokens > 1:
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        parts = [y.clone() for y in layer.forward_overlapped(x, streams, positions=positions)]
+        torch.cuda.synchronize()
+        h = tp.shard_range(tokens, 0, 2)[1]
+        assert torch.equal(parts[0], layer_by_hand(layer, x[:h], positions[:h], table, interleaved))
+        assert torch.equal(parts[1], layer_by_hand(layer, x[h:], positions[h:], table, interleaved))
+    g = torch.cuda.CUDAGraph()
+    xin, pin = x.clone(), positions.clone()
+    with torch.cuda.graph(g):
+        y = layer.forward(xin, positions=pin)
+    xin.copy_(rand(tokens, 512, seed=7, dtype=BF16))
+    pin.copy_(positions.flip(0))
+    g.replay()
+    assert torch.equal(y, layer_by_hand(layer, xin, pin, table, interleaved))
+
+
+def test_linear_out(cuda_device):
+    w, s = torch_ops.quantize_fp8(rand(300, 256, seed=1), layout="blocks")
+    x, bias = rand(40, 256, seed=2, dtype=BF16), rand(300, seed=3, dtype=BF16)
+    store = torch.full((40, 512), 7.0, device="cuda", dtype=BF16)
+    for lo in (0, 3, 100):
+        store.fill_(7.0)
+        out = torch_ops.linear_fp8_out(x, w, s, store[:, lo:lo + 300], bias)
+        assert torch.equal(out, torch_ops.linear_fp8(x, w, s, bias))
+        assert (store[:, :lo] == 7.0).all() and (store[:, lo + 300:] == 7.0).all()
+    for bad in (store, store[:, :300].float(), store[:39, :300]):
+        with pytest.raises(RuntimeError):
+            torch_ops.linear_fp8_out(x, w, s, bad, bias)

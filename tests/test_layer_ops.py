@@ -142,3 +142,38 @@ def test_no_gradient_is_refused():
                  lambda: torch_ops.rotary_(x, x, None, None)):
         with pytest.raises(RuntimeError, match="no gradient"):
             call()
+
+
+# ---------------------------------------------------------------- decoder layer
+
+
+def test_rotary_heads_of_a_shard():
+    from zcutlass_b200 import tp
+
+    s = tp.LLAMA3_8B  # 32 q, 8 k and 8 v heads of 128
+    assert tp.rotary_heads(s, 0, s.qkv_out) == 40
+    assert [tp.rotary_heads(s, *tp.shard_range(s.qkv_out, r, 4)) for r in range(4)] == [12, 12, 12, 4]
+    assert sum(tp.rotary_heads(s, *tp.shard_range(s.qkv_out, r, 8)) for r in range(8)) == 40
+    with pytest.raises(ValueError, match="whole heads"):
+        tp.rotary_heads(s, 64, 1024)
+    with pytest.raises(ValueError, match="whole heads"):
+        tp.rotary_heads(tp.QWEN2_1_5B, *tp.shard_range(tp.QWEN2_1_5B.qkv_out, 0, 5))
+
+
+def test_layer_positions_go_with_rotary():
+    from zcutlass_b200 import tp
+
+    def linear(x, w, bias, out):
+        out.copy_(x @ w.t())
+
+    layer = tp.TPDecoderLinears(tp.LayerShape(64, 128, 4, 2, 16), tp.TPGroup(), "cpu", torch.float32, linear_fn=linear)
+    x = torch.randn(5, 64)
+    y = layer.forward(x).clone()
+    with pytest.raises(ValueError, match="positions"):
+        layer.forward(x, positions=torch.arange(5))
+    with pytest.raises(ValueError, match="wider"):
+        layer.enable_rotary(torch.zeros(8, 32))
+    assert torch.equal(layer.forward(x), y)
+    layer.enable_rotary(torch_ops.rotary_table(8, 16))
+    with pytest.raises(ValueError, match="positions"):
+        layer.forward(x)

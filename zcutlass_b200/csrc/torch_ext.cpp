@@ -10,8 +10,8 @@
 //   torch.ops.zcutlass.linear(x, weight, bias=None) -> y
 //       nn.functional.linear semantics: weight is the PyTorch [N, K] layout and
 //       is consumed directly as a column-major B (no transposed copy).
-//   torch.ops.zcutlass.{quantize_fp8, gemm_fp8, linear_fp8, linear_fp8_train,
-//       rotary, rotary_}  8-bit block-scaled linears and
+//   torch.ops.zcutlass.{quantize_fp8, gemm_fp8, linear_fp8, linear_fp8_out,
+//       linear_fp8_train, rotary, rotary_}  8-bit block-scaled linears and
 //       rotary positions over the C ABI (documented in torch_ops.py)
 //
 // This file only adapts tensors to the library's entry points; all kernels live in libzcutlass.so.
@@ -275,12 +275,14 @@ void check_fp8_operand(const at::Tensor& t, const at::Tensor& scale, const char*
 
 at::Tensor run_gemm_fp8(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale,
                         const std::optional<at::Tensor>& bias, at::ScalarType out_type,
-                        at::IntArrayRef shape = {}) {
+                        at::IntArrayRef shape = {}, const at::Tensor& into = at::Tensor()) {
   const int64_t m = a.size(0), n = b.size(0), k = a.size(1);
-  at::Tensor d = shape.empty() ? empty_like_device({m, n}, out_type, a) : empty_like_device(shape, out_type, a);
+  at::Tensor d = into.defined()  ? into
+                 : shape.empty() ? empty_like_device({m, n}, out_type, a)
+                                 : empty_like_device(shape, out_type, a);
   zcutlass_fp8_gemm_desc g{};
   g.m = m, g.n = n, g.k = k;
-  g.lda = row_stride(a, "A"), g.ldb = row_stride(b, "B"), g.ldd = n;
+  g.lda = row_stride(a, "A"), g.ldb = row_stride(b, "B"), g.ldd = into.defined() ? row_stride(into, "out") : n;
   g.a_type = fp8_code(a.scalar_type(), "A"), g.b_type = fp8_code(b.scalar_type(), "B");
   g.d_type = float_code(d, "out_dtype");
   g.b_scale_rows = b_scale.size(0) == n ? 1 : 128;
@@ -331,6 +333,21 @@ at::Tensor linear_fp8_op(const at::Tensor& x, const at::Tensor& w, const at::Ten
   shape.back() = w.size(0);
   const Quantized r = quantize(as_rows(x), true, false, 1, at::kFloat8_e4m3fn, false);
   return run_gemm_fp8(r.q, r.scale, w, w_scale, bias, x.scalar_type(), shape);
+}
+
+void linear_fp8_out_op(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
+                       const std::optional<at::Tensor>& bias, at::Tensor out) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a rank-2 CUDA tensor");
+  (void)float_code(x, "x");
+  check_fp8_operand(w, w_scale, "weight", true);
+  TORCH_CHECK(x.device() == w.device() && out.device() == x.device(), "x, weight and out must be on the same CUDA device");
+  TORCH_CHECK(x.size(1) == w.size(1), "x.shape[1] must equal weight.shape[1]");
+  TORCH_CHECK(out.dim() == 2 && out.size(0) == x.size(0) && out.size(1) == w.size(0),
+              "out must be [x.shape[0], weight.shape[0]]");
+  TORCH_CHECK(out.scalar_type() == x.scalar_type(), "out dtype must match x");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Quantized r = quantize(as_rows(x), true, false, 1, at::kFloat8_e4m3fn, false);
+  run_gemm_fp8(r.q, r.scale, w, w_scale, bias, x.scalar_type(), {}, out);
 }
 
 // The differentiable linear keeps x and w in 8 bits, transposed, for its backward pass (undefined where the
@@ -568,6 +585,14 @@ at::Tensor linear_fp8_autograd(const at::Tensor& x, const at::Tensor& w, const a
   return linear_fp8_op(x, w, w_scale, bias);
 }
 
+void linear_fp8_out_autograd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
+                             const std::optional<at::Tensor>& bias, at::Tensor out) {
+  check_no_gradient("linear_fp8_out", x, w_scale, bias.value_or(at::Tensor()), out);
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  linear_fp8_out_op(x, w, w_scale, bias, out);
+  out.unsafeGetTensorImpl()->bump_version();
+}
+
 void rotary_inplace_autograd(at::Tensor q, at::Tensor k, const at::Tensor& positions, const at::Tensor& table,
                              bool interleaved, bool inverse) {
   TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k)),
@@ -594,6 +619,7 @@ TORCH_LIBRARY(zcutlass, m) {
   m.def("quantize_fp8(Tensor x, str layout=\"rows\", ScalarType? dtype=None) -> Tensor[]");
   m.def("gemm_fp8(Tensor A, Tensor A_scale, Tensor B, Tensor B_scale, Tensor? bias=None, ScalarType? out_dtype=None) -> Tensor");
   m.def("linear_fp8(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias=None) -> Tensor");
+  m.def("linear_fp8_out(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias, Tensor(a!) out) -> ()");
   m.def("linear_fp8_train(Tensor x, Tensor weight, Tensor? bias=None) -> Tensor");
   m.def("rotary(Tensor q, Tensor k, Tensor positions, Tensor table, bool interleaved=False, bool inverse=False) -> "
         "(Tensor, Tensor)");
@@ -608,6 +634,7 @@ TORCH_LIBRARY_IMPL(zcutlass, CUDA, m) {
   m.impl("quantize_fp8", quantize_fp8_op);
   m.impl("gemm_fp8", gemm_fp8_op);
   m.impl("linear_fp8", linear_fp8_op);
+  m.impl("linear_fp8_out", linear_fp8_out_op);
   m.impl("linear_fp8_train", linear_fp8_train_op);
   m.impl("rotary", rotary_op);
   m.impl("rotary_", rotary_inplace_op);
@@ -617,6 +644,7 @@ TORCH_LIBRARY_IMPL(zcutlass, Autograd, m) {
   m.impl("quantize_fp8", quantize_fp8_autograd);
   m.impl("gemm_fp8", gemm_fp8_autograd);
   m.impl("linear_fp8", linear_fp8_autograd);
+  m.impl("linear_fp8_out", linear_fp8_out_autograd);
   m.impl("linear_fp8_train", linear_fp8_train_autograd);
   m.impl("rotary", rotary_autograd);
   m.impl("rotary_", rotary_inplace_autograd);

@@ -8,6 +8,8 @@ Loading registers (CUDA dispatch key only):
     torch.ops.zcutlass.quantize_fp8(x, layout="rows", dtype=None) -> Tensor[]
     torch.ops.zcutlass.gemm_fp8(A, A_scale, B, B_scale, bias=None, out_dtype=None) -> D
     torch.ops.zcutlass.linear_fp8(x, weight, weight_scale, bias=None) -> y
+    torch.ops.zcutlass.linear_fp8_out(x, weight, weight_scale, bias, out) -> ()
+    torch.ops.zcutlass.linear_fp8_train(x, weight, bias=None) -> y   differentiable
     torch.ops.zcutlass.rotary(q, k, positions, table, interleaved=False, inverse=False) -> (q, k)
     torch.ops.zcutlass.rotary_(q, k, positions, table, ...) -> ()   in place
 
@@ -183,6 +185,13 @@ def linear_fp8(x, weight, weight_scale, bias=None):
     quantised by rows on the way in; y has x's dtype. For serving; training
     uses linear_fp8_train."""
     return _op("linear_fp8")(x, weight, weight_scale, bias)
+
+
+def linear_fp8_out(x, weight, weight_scale, out, bias=None):
+    """linear_fp8 of a matrix x [M, K] into out [M, N] (x's dtype, rows
+    contiguous, any row stride); returns out."""
+    _op("linear_fp8_out")(x, weight, weight_scale, bias, out)
+    return out
 
 
 def linear_fp8_train(x, weight, bias=None):

@@ -23,6 +23,11 @@ the linears, o_proj and down end in an NVLS reduce-scatter, and qkv / gate_up
 read the other ranks' rows inside the GEMM (zcutlass_gemm_gather_a: TMA loads
 from peer memory, no multicast), so no separate all-gather runs.
 
+TPDecoderLinears.quantize_fp8() turns the layer's weights into 8-bit floating
+point with 128 x 128 scales (linear_fp8 in torch_ops: activations quantised on
+the way in), and enable_rotary() applies rotary positions to the q and k heads
+of the qkv output in place; both are off unless called.
+
 Weights use the PyTorch [out_features, in_features] layout and go to the
 kernels as column-major B (no transposed copy). Every GEMM runs through the
 zcutlass C ABI (zcutlass_gemm) on the current stream; `linear_fn` replaces
@@ -79,11 +84,24 @@ def shard_range(total: int, rank: int, world: int) -> tuple[int, int]:
     return start, start + base + (1 if rank < rem else 0)
 
 
+class Fp8Weight:
+    """A [N, K] weight in 8-bit floating point with 128 x 128 scales, in the
+    place of a 16-bit one: `dtype` is that of the activations it works on."""
+
+    def __init__(self, weight) -> None:
+        self.q, self.scale = torch_ops.quantize_fp8(weight.detach(), layout="blocks")
+        self.shape, self.dtype, self.device = weight.shape, weight.dtype, weight.device
+
+
 def _linear_into(x, weight, bias, out) -> None:
     """out[M, N] = x[M, K] @ weight[N, K]^T (+ bias) through the zcutlass kernels."""
     import torch
 
     from . import _native
+
+    if isinstance(weight, Fp8Weight):
+        torch_ops.linear_fp8_out(x, weight.q, weight.scale, out, bias)
+        return
 
     torch_ops.load()
     m, k = x.shape
@@ -131,6 +149,8 @@ class ColumnParallelLinear:
 
         from . import _native
 
+        if isinstance(self.weight, Fp8Weight):
+            raise RuntimeError('the gathered GEMM reads 16-bit weights: use sp_gather = "copy" with 8-bit ones')
         k = self.weight.shape[1]
         n = self.weight.shape[0]
         t = _native.BF16 if self.weight.dtype == torch.bfloat16 else _native.F16
@@ -398,6 +418,19 @@ LLAMA3_70B = LayerShape(8192, 28672, 64, 8, 128)
 QWEN2_1_5B = LayerShape(1536, 8960, 12, 2, 128)
 
 
+def rotary_heads(shape: LayerShape, lo: int, hi: int) -> int:
+    """Heads of q and k in columns [lo, hi) of the packed q | k | v output: the
+    leading columns of that shard. The shard has to begin and end between
+    heads (or in v)."""
+    end = (shape.q_heads + shape.kv_heads) * shape.head_dim
+    if lo >= end:
+        return 0
+    width = min(hi, end) - lo
+    if lo % shape.head_dim or width % shape.head_dim:
+        raise ValueError(f"columns [{lo}, {hi}) of the qkv output cut a head of {shape.head_dim}: rotary positions need whole heads")
+    return width // shape.head_dim
+
+
 class TPDecoderLinears:
     """qkv / o_proj / gate_up / down of one layer, sharded over `tp`.
 
@@ -430,6 +463,8 @@ class TPDecoderLinears:
         self.down = RowParallelLinear(rnd(h, d_hi - d_lo, scale=inter ** -0.5), None, tp, chunks, linear_fn)
         self.o_cols = o_hi - o_lo
         self.d_cols = d_hi - d_lo
+        self._qkv_range = (qkv_lo, qkv_hi)
+        self.rotary_table = None  # set by enable_rotary()
         self._bufs = {}
         self.sp_inputs: list[NvlsReducer] = []  # set by enable_sequence_parallel()
         # How qkv / gate_up see the other ranks' rows in the sequence-parallel
@@ -438,6 +473,36 @@ class TPDecoderLinears:
         # (zcutlass_gemm_gather_a), which re-reads each remote A tile once per
         # N tile.
         self.sp_gather = "copy"
+
+    def quantize_fp8(self) -> None:
+        """Replaces the four weights by 8-bit ones (Fp8Weight), a quarter to a
+        half of the layer's memory traffic at decode and twice the tensor rate
+        at prefill. The 16-bit weights are dropped; idempotent."""
+        for linear in (self.qkv, self.o_proj, self.gate_up, self.down):
+            if not isinstance(linear.weight, Fp8Weight):
+                linear.weight = Fp8Weight(linear.weight)
+
+    def enable_rotary(self, table, interleaved: bool = False) -> None:
+        """Rotary positions on this rank's q and k heads, applied to the qkv
+        output in place, with a torch_ops.rotary_table on the layer's device
+        (its width is the rotary dimension). The forward calls then take
+        `positions`, one per row."""
+        if table.shape[1] > self.shape.head_dim:
+            raise ValueError("the table is wider than a head")
+        self._rotary_heads = rotary_heads(self.shape, *self._qkv_range)
+        self._rotary_interleaved = interleaved
+        self.rotary_table = table
+
+    def _check_positions(self, positions) -> None:
+        if (positions is None) != (self.rotary_table is None):
+            raise ValueError("positions are needed with enable_rotary(), and only then")
+
+    def _rotate(self, qkv, positions) -> None:
+        if positions is None or self._rotary_heads == 0:
+            return
+        heads = self._rotary_heads
+        qk = qkv[:, : heads * self.shape.head_dim].unflatten(1, (heads, self.shape.head_dim))
+        torch_ops.rotary_(qk, qk[:, :0], positions, self.rotary_table, self._rotary_interleaved)
 
     def enable_nvls(self, max_tokens: int, lanes: int = 1) -> bool:
         """Use the library's NVLS all-reduce for both row-parallel linears."""
@@ -460,7 +525,7 @@ class TPDecoderLinears:
         self.sp_inputs = made if int(ok.item()) == 1 else []
         return bool(self.sp_inputs)
 
-    def _sp_steps(self, rows: int, lane: int, xi: int, events: dict | None):
+    def _sp_steps(self, rows: int, lane: int, xi: int, events: dict | None, positions=None):
         """The sequence-parallel chain of one block of `rows` tokens, as two
         callables (through o_proj's reduce-scatter, then the rest). Rank r owns
         rows [r * rows / W, (r + 1) * rows / W) of the block: its input rows
@@ -469,6 +534,7 @@ class TPDecoderLinears:
         other ranks' rows as `sp_gather` says (copied into this rank's buffer,
         or read from the owners' buffers inside the GEMM); o_proj and down end
         in an NVLS reduce-scatter."""
+        self._check_positions(positions)
         b = self.buffers(rows, self.qkv.weight.device, self.qkv.weight.dtype, lane)
         x_in = self.sp_inputs[lane]
         state = {}
@@ -504,6 +570,7 @@ class TPDecoderLinears:
 
         def first():
             timed("qkv", lambda: gathered(self.qkv, x_in, xi, b["qkv"]))
+            self._rotate(b["qkv"], positions)
             timed("o_proj", o_proj)
 
         def second():
@@ -513,21 +580,23 @@ class TPDecoderLinears:
 
         return first, second, state
 
-    def forward_sp(self, rows: int, xi: int = 0, events: dict | None = None):
+    def forward_sp(self, rows: int, xi: int = 0, events: dict | None = None, positions=None):
         """Sequence-parallel layer step on lane 0 (see _sp_steps); returns the
         lane's down buffer, whose rows of this rank hold the result."""
-        first, second, state = self._sp_steps(rows, 0, xi, events)
+        first, second, state = self._sp_steps(rows, 0, xi, events, positions)
         first()
         second()
         return state["y"]
 
-    def forward_sp_overlapped(self, rows: int, streams, xi: int = 0):
+    def forward_sp_overlapped(self, rows: int, streams, xi: int = 0, positions=None):
         """forward_sp over len(streams) lanes, each a block of `rows` tokens in
-        its own input set, issued interleaved on their own streams."""
+        its own input set, issued interleaved on their own streams (positions:
+        one tensor per lane)."""
         import torch
 
         cur = torch.cuda.current_stream(self.qkv.weight.device)
-        chains = [self._sp_steps(rows, j, xi, None) for j in range(len(streams))]
+        chains = [self._sp_steps(rows, j, xi, None, None if positions is None else positions[j])
+                  for j in range(len(streams))]
         for s in streams:
             s.wait_stream(cur)
         for phase in (0, 1):
@@ -559,9 +628,10 @@ class TPDecoderLinears:
             }
         return self._bufs[key]
 
-    def _steps(self, x, lane: int, out, events: dict | None):
+    def _steps(self, x, lane: int, out, events: dict | None, positions=None):
         """The chain for one block of tokens, as two callables: up to and
         including o_proj's all-reduce, then gate_up, down and its all-reduce."""
+        self._check_positions(positions)
         b = self.buffers(x.shape[0], x.device, x.dtype, lane)
         state = {}
 
@@ -575,6 +645,7 @@ class TPDecoderLinears:
 
         def first():
             timed("qkv", lambda: self.qkv(x, b["qkv"]))
+            self._rotate(b["qkv"], positions)
             # o_proj input: this rank's heads of the attention output, stood in by the q part of qkv
             o_in = b["qkv"][:, : self.o_cols]
             # with NVLS the row-parallel outputs stay in their symmetric buffers (no copy)
@@ -590,18 +661,19 @@ class TPDecoderLinears:
 
         return first, second, state
 
-    def forward(self, x, events: dict | None = None, out=None):
+    def forward(self, x, events: dict | None = None, out=None, positions=None):
         """x: [tokens, hidden] (replicated on every rank). Runs the four GEMMs in
         a decoder layer's dependency order -- qkv, o_proj (+ all-reduce), gate_up
         on the o_proj output, down (+ all-reduce) -- and returns the down output
         (written into `out` when given). `events` (optional) maps a GEMM name to
-        a (start, end) CUDA event pair recorded around that GEMM on the current stream."""
-        first, second, state = self._steps(x, 0, out, events)
+        a (start, end) CUDA event pair recorded around that GEMM on the current stream.
+        `positions` (with enable_rotary): the position of each row of x."""
+        first, second, state = self._steps(x, 0, out, events, positions)
         first()
         second()
         return state["y"]
 
-    def forward_overlapped(self, x, streams, outs=None):
+    def forward_overlapped(self, x, streams, outs=None, positions=None):
         """The same layer over len(streams) independent blocks of rows of x (as
         from different sequences), each block's chain on its own stream and
         NVLS lane, issued interleaved so one block's all-reduce overlaps the
@@ -614,7 +686,8 @@ class TPDecoderLinears:
         chains = []
         for j in range(n):
             r0, r1 = shard_range(x.shape[0], j, n)
-            chains.append(self._steps(x[r0:r1], j, None if outs is None else outs[j], None))
+            chains.append(self._steps(x[r0:r1], j, None if outs is None else outs[j], None,
+                                      None if positions is None else positions[r0:r1]))
         for s in streams:
             s.wait_stream(cur)
         for phase in (0, 1):
@@ -625,7 +698,7 @@ class TPDecoderLinears:
             cur.wait_stream(s)
         return [c[2]["y"] for c in chains]
 
-    def forward_overlapped_layers(self, x, streams, layers: int, outs=None):
+    def forward_overlapped_layers(self, x, streams, layers: int, outs=None, positions=None):
         """`layers` consecutive layer steps over len(streams) independent row
         blocks, as a stack of decoder layers runs them: each block's chain of
         layers on its own stream and NVLS lane, the blocks joined only at the
@@ -644,7 +717,8 @@ class TPDecoderLinears:
             chains = []
             for j in range(n):
                 r0, r1 = shard_range(x.shape[0], j, n)
-                chains.append(self._steps(x[r0:r1], j, None if outs is None else outs[j], None))
+                chains.append(self._steps(x[r0:r1], j, None if outs is None else outs[j], None,
+                                      None if positions is None else positions[r0:r1]))
             for phase in (0, 1):
                 for j, s in enumerate(streams):
                     with torch.cuda.stream(s):
