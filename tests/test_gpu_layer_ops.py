@@ -587,3 +587,94 @@ def test_linear_out(cuda_device):
     for bad in (store, store[:, :300].float(), store[:39, :300]):
         with pytest.raises(RuntimeError):
             torch_ops.linear_fp8_out(x, w, s, bad, bias)
+
+
+# ---------------------------------------------------------------- second derivatives, first calls, calls at once
+
+
+def test_second_derivatives(cuda_device):
+    table = torch_ops.rotary_table(32, 32, device="cuda")
+    pos = torch.arange(9, device="cuda")
+    q, k = rand(9, 2, 32, seed=1).requires_grad_(), rand(9, 1, 32, seed=2).requires_grad_()
+    v = rand(9, 2, 32, seed=3).requires_grad_()
+    out, _ = torch_ops.rotary(q, k, pos, table)
+    (g,) = torch.autograd.grad(out, q, v, create_graph=True)
+    u = rand(9, 2, 32, seed=4)
+    (gg,) = torch.autograd.grad(g, v, u)  # the gradient is linear in v: its derivative turns u forward again
+    R.check_rotated(gg, u, pos, table, False)
+    x, w = rand(8, 64).requires_grad_(), rand(16, 64).requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(torch_ops.linear_fp8_train(x, w).sum(), x, create_graph=True)
+
+
+def test_backward_computes_what_is_asked(cuda_device):
+    """Gradients of one leaf alone, twice through one kept graph."""
+    x, w = rand(40, 256, seed=1, dtype=BF16).requires_grad_(), rand(128, 256, seed=2, dtype=BF16).requires_grad_()
+    dy = rand(40, 128, seed=3, dtype=BF16)
+    y = torch_ops.linear_fp8_train(x, w)
+    both = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(y, x, dy, retain_graph=True)[0], both[0])
+    assert torch.equal(torch.autograd.grad(y, w, dy)[0], both[1])
+
+
+def test_first_calls_inside_a_capture(cuda_device):
+    """A process whose first calls of every operator and kernel happen while a stream is captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from zcutlass_b200 import torch_ops as T
+x = torch.randn(600, 1024, device="cuda").bfloat16()
+big = torch.randn(2048, 1024, device="cuda")
+table = T.rotary_table(600, 128, device="cuda")
+pos = torch.arange(600, device="cuda")
+torch.cuda.synchronize()
+def step():
+    w, s = T.quantize_fp8(big, layout="blocks")
+    wr, sr = T.quantize_fp8(big, layout="rows")
+    out = [T.linear_fp8(x[:m], w, s) for m in (1, 20, 50, 300, 600)]
+    q, sq, _, _ = T.quantize_fp8(x, layout="both")
+    out += [T.gemm_fp8(q[:m], sq[:m], wr, sr) for m in (1, 20, 50, 300, 600)]
+    out += T.rotary(out[4][:, :1024].unflatten(1, (8, 128)), out[4][:, 1024:1280].unflatten(1, (2, 128)), pos, table)
+    return out
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    captured = step()
+g.replay()
+torch.cuda.synchronize()
+for a, b in zip(captured, step()):
+    assert torch.equal(a, b)
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_at_once_on_two_streams_and_threads(cuda_device):
+    """Every kernel of the product beside itself and the others, from two threads."""
+    import threading
+
+    w, s = torch_ops.quantize_fp8(rand(1536, 2048, seed=1, scale=0.03), layout="blocks")
+    xs = [rand(m, 2048, seed=m, dtype=BF16) for m in (1, 16, 30, 64, 200, 1500, 3000)]
+    want = [torch_ops.linear_fp8(x, w, s) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(order):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = [(i, torch_ops.linear_fp8(xs[i], w, s)) for i in order]
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(i for i, y in got if not torch.equal(y, want[i]))
+
+    threads = [threading.Thread(target=work, args=(o,)) for o in (range(7), range(6, -1, -1))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    from zcutlass_b200 import _native
+
+    assert _native.device_error() == 0
