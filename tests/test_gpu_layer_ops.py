@@ -678,3 +678,36 @@ def test_calls_at_once_on_two_streams_and_threads(cuda_device):
     from zcutlass_b200 import _native
 
     assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("xt", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("m", [1, 3, 15, 16])
+@pytest.mark.parametrize("k", [1, 100, 128, 130, 1000, 4096, 4200])
+def test_linear_of_few_rows_has_the_bits_of_quantise_then_product(cuda_device, m, k, xt):
+    """Odd widths, unaligned and strided rows, an infinity that stays in its row."""
+    w, s = torch_ops.quantize_fp8(rand(390, k, seed=1, scale=k ** -0.5), layout="blocks")
+    bias = rand(390, seed=2, dtype=xt)
+    for x in (rand(m, k, seed=3, dtype=xt), rand(m, k + 9, seed=4, dtype=xt)[:, 3:3 + k], rand(2 * m, k + 8, seed=5, dtype=xt)[::2, :k]):
+        q, sx = torch_ops.quantize_fp8(x.contiguous())
+        want = torch_ops.gemm_fp8(q, sx, w, s, bias, xt)
+        assert torch.equal(torch_ops.linear_fp8(x, w, s, bias), want)
+    if m > 1:
+        x = rand(m, k, seed=6, dtype=xt)
+        x[1, k // 2] = float("inf")
+        y = torch_ops.linear_fp8(x, w, s)
+        assert torch.isnan(y[1]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all()
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 8])
+def test_linear_of_few_rows_splits(cuda_device, monkeypatch, splits):
+    monkeypatch.setenv("ZCUTLASS_SPLITK", str(splits))
+    w, s = torch_ops.quantize_fp8(rand(256, 2500, seed=1, scale=0.02), layout="blocks")
+    check_linear(rand(9, 2500, seed=2, dtype=BF16), w, s, None)
+
+
+def test_linear_of_few_rows_with_unaligned_weights(cuda_device):
+    w, s = torch_ops.quantize_fp8(rand(200, 333, seed=1, scale=0.05), layout="blocks")
+    packed = w.view(torch.uint8).contiguous().view(E4M3)  # rows of 333 bytes: the generic kernel
+    check_linear(rand(5, 333, seed=2, dtype=BF16), packed, s, None)
+    w, s = torch_ops.quantize_fp8(rand(200, 256, seed=1, scale=0.05), layout="rows")  # a scale per row
+    check_linear(rand(5, 256, seed=2, dtype=BF16), w, s, None)

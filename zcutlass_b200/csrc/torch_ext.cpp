@@ -273,28 +273,29 @@ void check_fp8_operand(const at::Tensor& t, const at::Tensor& scale, const char*
               blocks_allowed ? "rows or ceil(rows / 128)" : "rows", ", ceil(columns / 128)] of ", name);
 }
 
+const void* bias_ptr(const std::optional<at::Tensor>& bias, const at::Tensor& a, at::ScalarType out_type, int64_t n) {
+  if (!bias.has_value()) return nullptr;
+  TORCH_CHECK(bias->is_cuda() && bias->device() == a.device() && bias->dim() == 1 && bias->is_contiguous(),
+              "bias must be a contiguous rank-1 CUDA tensor on the operands' device");
+  TORCH_CHECK(bias->scalar_type() == out_type, "bias dtype must match the result's");
+  TORCH_CHECK(bias->size(0) == n, "bias length must equal B.shape[0]");
+  return bias->data_ptr();
+}
+
 at::Tensor run_gemm_fp8(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale,
                         const std::optional<at::Tensor>& bias, at::ScalarType out_type,
-                        at::IntArrayRef shape = {}, const at::Tensor& into = at::Tensor()) {
+                        at::IntArrayRef shape = {}) {
   const int64_t m = a.size(0), n = b.size(0), k = a.size(1);
-  at::Tensor d = into.defined()  ? into
-                 : shape.empty() ? empty_like_device({m, n}, out_type, a)
-                                 : empty_like_device(shape, out_type, a);
+  at::Tensor d = shape.empty() ? empty_like_device({m, n}, out_type, a) : empty_like_device(shape, out_type, a);
   zcutlass_fp8_gemm_desc g{};
   g.m = m, g.n = n, g.k = k;
-  g.lda = row_stride(a, "A"), g.ldb = row_stride(b, "B"), g.ldd = into.defined() ? row_stride(into, "out") : n;
+  g.lda = row_stride(a, "A"), g.ldb = row_stride(b, "B"), g.ldd = n;
   g.a_type = fp8_code(a.scalar_type(), "A"), g.b_type = fp8_code(b.scalar_type(), "B");
   g.d_type = float_code(d, "out_dtype");
   g.b_scale_rows = b_scale.size(0) == n ? 1 : 128;
   g.a_scale_row = a_scale.stride(0), g.a_scale_blk = a_scale.stride(1);
   g.b_scale_row = b_scale.stride(0), g.b_scale_blk = b_scale.stride(1);
-  if (bias.has_value()) {
-    TORCH_CHECK(bias->is_cuda() && bias->device() == a.device() && bias->dim() == 1 && bias->is_contiguous(),
-                "bias must be a contiguous rank-1 CUDA tensor on the operands' device");
-    TORCH_CHECK(bias->scalar_type() == out_type, "bias dtype must match the result's");
-    TORCH_CHECK(bias->size(0) == n, "bias length must equal B.shape[0]");
-    g.bias = bias->data_ptr();
-  }
+  g.bias = bias_ptr(bias, a, out_type, n);
   g.stream = current_stream();
   check_status(zcutlass_gemm_fp8(&g, a.data_ptr(), a_scale.data_ptr<float>(), b.data_ptr(), b_scale.data_ptr<float>(),
                                  d.data_ptr()),
@@ -310,6 +311,35 @@ at::Tensor gemm_fp8_op(const at::Tensor& a, const at::Tensor& a_scale, const at:
   TORCH_CHECK(a.size(1) == b.size(1), "A.shape[1] must equal B.shape[1]");
   const c10::cuda::CUDAGuard guard(a.device());
   return run_gemm_fp8(a, a_scale, b, b_scale, bias, out_dtype.value_or(at::kBFloat16));
+}
+
+// y = x w^T + bias for a matrix x of rows. The quantised x and its scales share one allocation and never
+// become tensors: at decode, the calls around two short kernels are most of the time.
+at::Tensor run_linear_fp8(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
+                          const std::optional<at::Tensor>& bias, at::IntArrayRef shape, const at::Tensor& into) {
+  const int64_t m = x.size(0), n = w.size(0), k = x.size(1);
+  const int64_t ldq = (k + 15) / 16 * 16, q_bytes = m * ldq;
+  const at::Tensor buffer = empty_like_device({q_bytes + 4 * m * groups(k)}, at::kByte, x);
+  uint8_t* const q = static_cast<uint8_t*>(buffer.data_ptr());
+  float* const scale = reinterpret_cast<float*>(q + q_bytes);
+  zcutlass_quantize_desc d{};
+  d.rows = m, d.cols = k, d.ldx = row_stride(x, "x");
+  d.x_type = float_code(x, "x"), d.q_type = ZCUTLASS_E4M3, d.block_rows = 1;
+  d.ldq = ldq, d.scale_row = 1, d.scale_blk = m;
+  d.stream = current_stream();
+  const at::Tensor y = into.defined() ? into : empty_like_device(shape, x.scalar_type(), x);
+  zcutlass_fp8_gemm_desc g{};
+  g.m = m, g.n = n, g.k = k;
+  g.lda = ldq, g.ldb = row_stride(w, "weight"), g.ldd = into.defined() ? row_stride(into, "out") : n;
+  g.a_type = ZCUTLASS_E4M3, g.b_type = fp8_code(w.scalar_type(), "weight"), g.d_type = d.x_type;
+  g.b_scale_rows = w_scale.size(0) == n ? 1 : 128;
+  g.a_scale_row = 1, g.a_scale_blk = m;
+  g.b_scale_row = w_scale.stride(0), g.b_scale_blk = w_scale.stride(1);
+  g.bias = bias_ptr(bias, x, x.scalar_type(), n);
+  g.stream = d.stream;
+  check_status(zcutlass_quantize_fp8(&d, x.data_ptr(), q, scale, nullptr, nullptr, nullptr), "zcutlass_quantize_fp8");
+  check_status(zcutlass_gemm_fp8(&g, q, scale, w.data_ptr(), w_scale.data_ptr<float>(), y.data_ptr()), "zcutlass_gemm_fp8");
+  return y;
 }
 
 // x as a matrix [rows, last dimension] of contiguous rows (a copy only where its strides leave no other way).
@@ -331,8 +361,7 @@ at::Tensor linear_fp8_op(const at::Tensor& x, const at::Tensor& w, const at::Ten
   const c10::cuda::CUDAGuard guard(x.device());
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = w.size(0);
-  const Quantized r = quantize(as_rows(x), true, false, 1, at::kFloat8_e4m3fn, false);
-  return run_gemm_fp8(r.q, r.scale, w, w_scale, bias, x.scalar_type(), shape);
+  return run_linear_fp8(as_rows(x), w, w_scale, bias, shape, at::Tensor());
 }
 
 void linear_fp8_out_op(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
@@ -346,8 +375,7 @@ void linear_fp8_out_op(const at::Tensor& x, const at::Tensor& w, const at::Tenso
               "out must be [x.shape[0], weight.shape[0]]");
   TORCH_CHECK(out.scalar_type() == x.scalar_type(), "out dtype must match x");
   const c10::cuda::CUDAGuard guard(x.device());
-  const Quantized r = quantize(as_rows(x), true, false, 1, at::kFloat8_e4m3fn, false);
-  run_gemm_fp8(r.q, r.scale, w, w_scale, bias, x.scalar_type(), {}, out);
+  run_linear_fp8(as_rows(x), w, w_scale, bias, {}, out);
 }
 
 // The differentiable linear keeps x and w in 8 bits, transposed, for its backward pass (undefined where the
