@@ -126,14 +126,19 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return d;
 }
 
-// acc += (s * scale) * r for one 16 x 32 step of fragments: column scales s at sb (every fourth pair), row
-// scales lo and hi of the fragment's two rows.
-__device__ __forceinline__ void add_fragments(float* acc, const uint32_t (&r)[16], const float2* sb, float lo, float hi) {
+// The four pairs of column scales that a thread meets in 32 columns, from `sb` (its pair of the first group).
+__device__ __forceinline__ void load_column_scales(float2 (&s)[4], const float2* sb) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) s[g] = sb[g * 4];
+}
+
+// acc += (s * scale) * r for one 16 x 32 step of fragments: column scales s, row scales lo and hi of the
+// fragment's two rows.
+__device__ __forceinline__ void add_fragments(float* acc, const uint32_t (&r)[16], const float2 (&s)[4], float lo, float hi) {
   const uint64_t lo2 = pack2(lo, lo), hi2 = pack2(hi, hi);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const float2 s = sb[g * 4];
-    const uint64_t s2 = pack2(s.x, s.y);
+    const uint64_t s2 = pack2(s[g].x, s[g].y);
     float* q = acc + 4 * g;
     const float2 a = unpack2(fma2(mul2(s2, lo2), pack2(__uint_as_float(r[4 * g]), __uint_as_float(r[4 * g + 1])), pack2(q[0], q[1])));
     const float2 b = unpack2(fma2(mul2(s2, hi2), pack2(__uint_as_float(r[4 * g + 2]), __uint_as_float(r[4 * g + 3])), pack2(q[2], q[3])));

@@ -335,19 +335,23 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) sa[j] = slot[quarter * 32 + j * 8 + (lane >> 2)];
           const float2* sb = reinterpret_cast<const float2*>(slot + kHalf + half * kHalf) + (lane & 3);
+          float2 cs[2][4];  // column scales, loaded two steps ahead
+          fp8::load_column_scales(cs[0], sb);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {  // 32 columns of 16 rows per step: (c / 2, c % 2)
             uint32_t(&r)[16] = v[c & 1];
+            if (c % 2 == 0 && c < 6) fp8::load_column_scales(cs[(c / 2 + 1) & 1], sb + (c / 2 + 1) * 16);
             fp8::tmem_ld_wait_x16(r);
             if (c + 1 < 8) {
               fp8::tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, v[(c + 1) & 1]);
             } else {
+              // The slot has been read, too: the last column scales were used in the step before.
               tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
             }
-            fp8::add_fragments(acc + (c >> 1) * 32 + (c & 1) * 16, r, sb + (c >> 1) * 16, sa[2 * (c & 1)], sa[2 * (c & 1) + 1]);
+            fp8::add_fragments(acc + (c >> 1) * 32 + (c & 1) * 16, r, cs[(c / 2) & 1], sa[2 * (c & 1)], sa[2 * (c & 1) + 1]);
           }
-          __syncwarp();  // the slot has been read, too
-          if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
         }
       }
       if (!ok) break;

@@ -275,26 +275,31 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
       load(0, v[0]);
       const float mine = kSwap ? (kRows ? slot[TM + row] : 1.0f) : (kFragments ? 1.0f : slot[row]);
       float lo_hi[4];
+      float2 cs[2][4];  // column scales, loaded two steps ahead
+      const float2* sb = reinterpret_cast<const float2*>(slot + TM) + (lane & 3);
       if constexpr (kFragments) {
+        fp8::load_column_scales(cs[0], sb);
 #pragma unroll
         for (int j = 0; j < 4; ++j) lo_hi[j] = slot[quarter * 32 + j * 8 + (lane >> 2)];
       }
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
         uint32_t(&r)[16] = v[c & 1];
+        if constexpr (kFragments) {
+          if (c % 2 == 0 && c + 2 < kSteps) fp8::load_column_scales(cs[(c / 2 + 1) & 1], sb + (c / 2 + 1) * 16);
+        }
         fp8::tmem_ld_wait_x16(r);
         if (c + 1 < kSteps) {
           load(c + 1, v[(c + 1) & 1]);
         } else {
           tc_fence_before_sync();
-          if constexpr (!kSwap && !kFragments) {  // nothing of the slot is read after this
+          if constexpr (!kSwap) {  // nothing of the slot is read after this (fragments: two steps ahead)
             __syncwarp();
             if (lane == 0) mbar_arrive(&tmem_empty[buf]);
           }
         }
         if constexpr (kFragments) {
-          const float2* sb = reinterpret_cast<const float2*>(slot + TM) + (lane & 3);
-          fp8::add_fragments(acc + (c >> 1) * 32 + (c & 1) * 16, r, sb + (c >> 1) * 16, lo_hi[2 * (c & 1)], lo_hi[2 * (c & 1) + 1]);
+          fp8::add_fragments(acc + (c >> 1) * 32 + (c & 1) * 16, r, cs[(c / 2) & 1], lo_hi[2 * (c & 1)], lo_hi[2 * (c & 1) + 1]);
         } else if constexpr (kSwap) {
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
           for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(mine, __uint_as_float(r[j]), acc[c * 16 + j]);
         }
       }
-      if constexpr (kSwap || kFragments) {
+      if constexpr (kSwap) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&tmem_empty[buf]);
       }
