@@ -195,25 +195,60 @@ bool any_forced() {
   return f != nullptr && std::strncmp(f, "fp8_", 4) == 0;
 }
 
+// Clusters of `size` CTAs of the 128 x 128 tile kernel (one CTA per SM) that run at once: clusters stay within
+// a GPC, so 148 SMs hold 74, 45, 33, 26, 22, 15 and 15 of 2 to 8. Asked once per device and size.
+int resident_clusters(const DeviceInfo& dev, int size) {
+  if (size == 1) return dev.sm_count;
+  static std::atomic<int> known[64][fp8_tile::kMaxSplits + 1];
+  std::atomic<int>& slot = known[dev.ordinal & 63][size];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  auto kernel = fp8_tile::gemm_kernel<false, 128, false, 3, 2>;
+  constexpr int kBytes = fp8_tile::Smem<false, 128, false, 3, 2>::kDynamicBytes;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(size), 1, 1);
+  cfg.blockDim = dim3(fp8_tile::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kBytes;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(size);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+    (void)cudaGetLastError();
+    n = dev.sm_count / (2 * size);
+  }
+  slot.store(n, std::memory_order_relaxed);
+  return n;
+}
+
 // CTAs along K per tile, each with at least two blocks, at most a cluster of 8. The swapped kernel, two CTAs
 // of which fit an SM: the power of two that gives (nearly) every SM one, since more only add partial tiles to
 // exchange, and clusters of other sizes leave SMs out: 16 x 4096 x 4096 (32 tiles) takes 8.3, 6.5 and 7.6 us
 // with 2, 4 and 8 splits, 1 x 6144 x 4096 (48 tiles) 8.6, 8.4, 7.4, 8.5 and 12.1 with 2, 3, 4, 5 and 6. The
-// other, one CTA of which fills an SM: as many as run at once.
-int tile_splits(int64_t tiles, int64_t num_kb, int64_t sms, bool swap) {
+// other, one CTA of which fills an SM: as many as run at once (200 x 1024 x 4096, 16 tiles: 13.3 us with 8
+// splits in two waves).
+int tile_splits(int64_t tiles, int64_t num_kb, const DeviceInfo& dev, bool swap) {
   const char* v = std::getenv("ZCUTLASS_SPLITK");
-  int64_t s = sms / tiles;
-  if (swap)
-    for (s = 1; s < fp8_tile::kMaxSplits && s * tiles < sms * 6 / 7; s *= 2) {}
-  if (v != nullptr && v[0] != '\0') s = std::atoi(v);
-  s = std::min<int64_t>(s, std::min<int64_t>(fp8_tile::kMaxSplits, num_kb / 2));
-  return static_cast<int>(std::max<int64_t>(s, 1));
+  const int most = static_cast<int>(std::min<int64_t>(fp8_tile::kMaxSplits, num_kb / 2));
+  int s = 1;
+  if (v != nullptr && v[0] != '\0') {
+    s = std::atoi(v);
+  } else if (swap) {
+    while (s < most && s * tiles < dev.sm_count * 6 / 7) s *= 2;
+  } else {
+    for (s = most; s > 1 && tiles > resident_clusters(dev, s); --s) {}
+  }
+  return std::max(1, std::min(s, most));
 }
 
 cudaError_t tensor_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, cudaStream_t stream) {
   const int64_t tiles_n = div_up(g.n, 128), kb = div_up(g.k, fp8::kBlockK), sms = dev.sm_count;
   const bool any = any_forced();
-  const auto splits = [&](int tm) { return tile_splits(tiles_n * div_up(g.m, tm), kb, sms, tm < 128); };
+  const auto splits = [&](int tm) { return tile_splits(tiles_n * div_up(g.m, tm), kb, dev, tm < 128); };
   // Where there is no more than a CTA per SM, one with two blocks per stage and the SM's whole shared memory
   // streams faster than one made for two per SM (48 x 4096 x 14336: 15.6 against 17.1 us; with 224 CTAs,
   // 64 x 28672 x 4096, 30.8 against 23.2). 16 rows are served by the same ring both ways.
