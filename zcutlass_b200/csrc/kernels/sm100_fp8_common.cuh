@@ -126,6 +126,41 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return d;
 }
 
+// The same for registers already waited for.
+__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+
+// acc += scale() * (128 columns of this thread's TMEM lane at t0); `read_done` is called when the last column has
+// been read. Two loads of 32 columns are in flight at a time: eight of 16, one ahead, held the buffer 3 % of a
+// product longer.
+template <typename Scale, typename ReadDone>
+__device__ __forceinline__ void add_columns(float (&acc)[128], uint32_t t0, Scale scale, ReadDone read_done) {
+  uint32_t a[32], b[32];
+  tmem_ld_32x32b_x32(t0, a);
+  tmem_ld_32x32b_x32(t0 + 32, b);
+  const float s = scale();  // from shared memory while the loads are on their way
+  tmem_ld_wait();
+  after_wait(a);
+  after_wait(b);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) acc[j] = fmaf(s, __uint_as_float(a[j]), acc[j]);
+  tmem_ld_32x32b_x32(t0 + 64, a);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) acc[32 + j] = fmaf(s, __uint_as_float(b[j]), acc[32 + j]);
+  tmem_ld_32x32b_x32(t0 + 96, b);
+  tmem_ld_wait();
+  after_wait(a);
+  after_wait(b);
+  read_done();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) acc[64 + j] = fmaf(s, __uint_as_float(a[j]), acc[64 + j]);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) acc[96 + j] = fmaf(s, __uint_as_float(b[j]), acc[96 + j]);
+}
+
 // The four pairs of column scales that a thread meets in 32 columns, from `sb` (its pair of the first group).
 __device__ __forceinline__ void load_column_scales(float2 (&s)[4], const float2* sb) {
 #pragma unroll

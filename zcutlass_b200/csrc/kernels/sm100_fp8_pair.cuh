@@ -104,6 +104,59 @@ __device__ __forceinline__ void raster(int tile, const Fp8PairParams& p, int& tm
   tn = in / rows;
 }
 
+// Four chunks of 32 rows x 64 bytes, in the 64-byte swizzle that the stores to D expect, from a warp's
+// accumulators (all 128 columns of a 16-bit type, 64 of a 32-bit one).
+template <bool kRows, int kType>
+__device__ __forceinline__ void fill(uint8_t* out, const float* acc, int lane) {
+  constexpr bool kWide = kType == fp8::kF32;
+  if constexpr (!kRows) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint4* row = reinterpret_cast<uint4*>(out + c * 2048 + lane * 64);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint4 word;
+        if constexpr (kWide) {
+          const float* f = acc + 16 * c + 4 * q;
+          word = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        } else {
+          const float* f = acc + 32 * c + 8 * q;
+          word = make_uint4(fp8::pack_out(f[0], f[1], kType), fp8::pack_out(f[2], f[3], kType), fp8::pack_out(f[4], f[5], kType),
+                            fp8::pack_out(f[6], f[7], kType));
+        }
+        row[q ^ ((lane >> 1) & 3)] = word;
+      }
+    }
+  } else {
+    // Value j of 32: rows 16 (j / 16) + 8 (j % 4 / 2) + lane / 4, columns 8 (j / 4 % 4) + 2 (lane % 4) and the next.
+#pragma unroll
+    for (int j = 0; j < (kWide ? 64 : 128); j += 2) {
+      const int row = 16 * ((j >> 4) & 1) + 8 * ((j >> 1) & 1) + (lane >> 2);
+      const int g = (j >> 2) & 3;
+      if constexpr (kWide) {
+        const int c = 2 * (j >> 5) + (g >> 1), unit = 2 * (g & 1) + ((lane & 3) >> 1);
+        *reinterpret_cast<float2*>(out + c * 2048 + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4) + (lane & 1) * 8) =
+            make_float2(acc[j], acc[j + 1]);
+      } else {
+        *reinterpret_cast<uint32_t*>(out + (j >> 5) * 2048 + row * 64 + ((g ^ ((row >> 1) & 3)) << 4) + (lane & 3) * 4) =
+            fp8::pack_out(acc[j], acc[j + 1], kType);
+      }
+    }
+  }
+}
+
+// Stores the four chunks (kCols columns each) at column n of rows m..m + 31.
+template <int kCols>
+__device__ __forceinline__ void flush(const uint8_t* out, const CUtensorMap* map, int n, int m, int lane) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tma_store_2d(map, out + c * 2048, n + c * kCols, m);
+    bulk_commit_group();
+  }
+}
+
 template <bool kRows>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -290,7 +343,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* out = smem + L::kOutOff + w * L::kOutWarp;
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * kHalf;
     uint32_t i = 0;
-    uint32_t chunk = 0;
     bool ok = true;
     for (int tile = pair; ok && tile < p.total_tiles; tile += npairs) {
       int tm, tn;
@@ -310,26 +362,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after_sync();
-        uint32_t v[2][16];
         const uint32_t t0 = taddr + buf * kBlock;
+        const auto read_done = [&] {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
+        };
         if constexpr (!kRows) {
-          fp8::tmem_ld_x16(t0, v[0]);
-          const float scale = slot[quarter * 32 + lane] * slot[kHalf + half];
-#pragma unroll
-          for (int c = 0; c < kHalf / 16; ++c) {
-            uint32_t(&r)[16] = v[c & 1];
-            fp8::tmem_ld_wait_x16(r);
-            if (c + 1 < kHalf / 16) {
-              fp8::tmem_ld_x16(t0 + (c + 1) * 16, v[(c + 1) & 1]);
-            } else {
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(scale, __uint_as_float(r[j]), acc[c * 16 + j]);
-          }
+          fp8::add_columns(acc, t0, [&] { return slot[quarter * 32 + lane] * slot[kHalf + half]; }, read_done);
         } else {
+          uint32_t v[2][16];
           fp8::tmem_ld_16x256b_x4(t0, v[0]);
           float sa[4];
 #pragma unroll
@@ -345,81 +387,50 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (c + 1 < 8) {
               fp8::tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, v[(c + 1) & 1]);
             } else {
-              // The slot has been read, too: the last column scales were used in the step before.
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
+              read_done();  // of the slot, too: the last column scales were used in the step before
             }
             fp8::add_fragments(acc + (c >> 1) * 32 + (c & 1) * 16, r, cs[(c / 2) & 1], sa[2 * (c & 1)], sa[2 * (c & 1) + 1]);
           }
         }
       }
       if (!ok) break;
-      // Chunks of 32 rows x 64 bytes (32 values of 16 bits, 16 of 32) go out by TMA, four in flight.
-      const bool wide = p.d_type == fp8::kF32;
+      if (n0 >= p.n || m0 >= p.m) continue;
+      if (p.bias != nullptr) {
 #pragma unroll
-      for (int c = 0; c < kHalf / 32; ++c) {
-        const int nc = n0 + c * 32;
-        if (nc >= p.n || m0 >= p.m) break;
-        float* v = acc + c * 32;
-        if (p.bias != nullptr) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int col = kRows ? 8 * ((j >> 2) & 3) + 2 * (lane & 3) + (j & 1) : j;
-            if (nc + col < p.n) v[j] += fp8::load_out(p.bias, nc + col, p.d_type);
-          }
+        for (int j = 0; j < kHalf; ++j) {
+          const int col = kRows ? 32 * (j >> 5) + 8 * ((j >> 2) & 3) + 2 * (lane & 3) + (j & 1) : j;
+          if (n0 + col < p.n) acc[j] += fp8::load_out(p.bias, n0 + col, p.d_type);
         }
-        if (p.tma_d && nc + 32 <= p.n) {
+      }
+      if (p.tma_d && n0 + kHalf <= p.n) {
+        // Chunks of 32 rows x 64 bytes (32 values of 16 bits, 16 of 32), four at a time: one fence and one group
+        // of stores for all (a fence per chunk made the output 3000 cycles per tile, as long as four k blocks).
+        if (p.d_type == fp8::kF32) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h == 1 && !wide) break;
-            uint8_t* buf = out + (chunk & 3u) * 2048;
-            if (lane == 0) bulk_wait_group_read<3>();
+          for (int round = 0; round < 2; ++round) {
+            if (lane == 0) bulk_wait_group_read<0>();
             __syncwarp();
-            if constexpr (!kRows) {
-              uint4* row = reinterpret_cast<uint4*>(buf + lane * 64);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint4 word;
-                if (wide) {
-                  const float* f = v + h * 16 + 4 * q;
-                  word = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-                } else {
-                  const float* f = v + 8 * q;
-                  word = make_uint4(fp8::pack_out(f[0], f[1], p.d_type), fp8::pack_out(f[2], f[3], p.d_type),
-                                    fp8::pack_out(f[4], f[5], p.d_type), fp8::pack_out(f[6], f[7], p.d_type));
-                }
-                row[q ^ ((lane >> 1) & 3)] = word;
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {  // rows 16 (j / 16) + 8 (j % 4 / 2) + lane / 4, group j / 4 % 4
-                const int row = 16 * (j >> 4) + 8 * ((j >> 1) & 1) + (lane >> 2);
-                const int g = (j >> 2) & 3;
-                if (wide) {
-                  if ((g >> 1) != h) continue;
-                  const int unit = 2 * (g & 1) + ((lane & 3) >> 1);  // 16 bytes: 4 columns
-                  *reinterpret_cast<float2*>(buf + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4) + (lane & 1) * 8) =
-                      make_float2(v[j], v[j + 1]);
-                } else {
-                  *reinterpret_cast<uint32_t*>(buf + row * 64 + ((g ^ ((row >> 1) & 3)) << 4) + (lane & 3) * 4) =
-                      fp8::pack_out(v[j], v[j + 1], p.d_type);
-                }
-              }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&tmap_d, buf, nc + h * 16, m0);
-              bulk_commit_group();
-            }
-            ++chunk;
+            fill<kRows, fp8::kF32>(out, acc + round * 64, lane);
+            flush<16>(out, &tmap_d, n0 + round * 64, m0, lane);
           }
         } else {
-          // Ragged or unaligned: through shared memory as 32-bit values, then whole rows of 32 columns.
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
-          float* stage = reinterpret_cast<float*>(out);
+          if (p.d_type == fp8::kBf16) fill<kRows, fp8::kBf16>(out, acc, lane);
+          else fill<kRows, fp8::kF16>(out, acc, lane);
+          flush<32>(out, &tmap_d, n0, m0, lane);
+        }
+      } else {
+        // Ragged or unaligned: through shared memory as 32-bit values, then whole rows of 32 columns.
+        if (lane == 0) bulk_wait_group_read<0>();
+        float* stage = reinterpret_cast<float*>(out);
+        const int rows = p.m - m0 < 32 ? p.m - m0 : 32;
+#pragma unroll
+        for (int c = 0; c < kHalf / 32; ++c) {
+          const int nc = n0 + c * 32;
+          if (nc >= p.n) break;
+          __syncwarp();
+          const float* v = acc + c * 32;
           if constexpr (!kRows) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
@@ -434,14 +445,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           __syncwarp();
-          const int rows = p.m - m0 < 32 ? p.m - m0 : 32;
           if (nc + lane < p.n) {
             for (int r = 0; r < rows; ++r)
               fp8::store_out(p.d, static_cast<int64_t>(m0 + r) * p.ldd + nc + lane, p.d_type,
                              stage[r * 32 + 4 * ((lane >> 2) ^ (r & 7)) + (lane & 3)]);
           }
-          __syncwarp();
         }
+        __syncwarp();
       }
     }
     if (lane == 0) bulk_wait_group<0>();

@@ -267,13 +267,22 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
       if (!ok) break;
       tc_fence_after_sync();
       const uint32_t t0 = taddr + buf * L::kMmaN;
+      if constexpr (!kSwap && !kRows) {
+        fp8::add_columns(acc, t0, [&] { return slot[row]; }, [&] {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tmem_empty[buf]);
+        });
+        if (++buf == kBufs) buf = 0, phase ^= 1u;
+        continue;
+      }
       uint32_t v[2][16];
       auto load = [&](int c, uint32_t(&r)[16]) {
         if constexpr (kFragments) fp8::tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>(c & 1) * 16) << 16) + (c >> 1) * 32, r);
         else fp8::tmem_ld_x16(t0 + c * 16, r);
       };
       load(0, v[0]);
-      const float mine = kSwap ? (kRows ? slot[TM + row] : 1.0f) : (kFragments ? 1.0f : slot[row]);
+      const float mine = kSwap && kRows ? slot[TM + row] : 1.0f;
       float lo_hi[4];
       float2 cs[2][4];  // column scales, loaded two steps ahead
       const float2* sb = reinterpret_cast<const float2*>(slot + TM) + (lane & 3);
@@ -309,9 +318,6 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
             for (int q = 0; q < 4; ++q)
               acc[c * 16 + j + q] = fmaf(kRows ? f[q] * mine : f[q], __uint_as_float(r[j + q]), acc[c * 16 + j + q]);
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(mine, __uint_as_float(r[j]), acc[c * 16 + j]);
         }
       }
       if constexpr (kSwap) {
