@@ -17,7 +17,10 @@
 // With a scale per row of B (kRows) it is a factor per thread (kSwap), or TMEM is
 // read as 16 x 8 fragments, in which a thread meets 32 of 128 columns.
 //
-// Bound by bytes: a stage of the TMA ring holds KSUB blocks. The splits' 32-bit
+// Bound by bytes: a stage of the TMA ring holds KSUB = 2 blocks. The same bytes
+// in stages of one block: 512 x 4096 x 4096 20.2 us against 16.9, 1 x 6144 x 4096
+// 8.2 against 8.4 (3 splits); half the ring: 48 x 4096 x 14336 17.1-17.3 against
+// 15.6 with either. The splits' 32-bit
 // partial tiles are added in split order through distributed shared memory, so
 // the result does not depend on timing.
 #pragma once
@@ -267,22 +270,13 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
       if (!ok) break;
       tc_fence_after_sync();
       const uint32_t t0 = taddr + buf * L::kMmaN;
-      if constexpr (!kSwap && !kRows) {
-        fp8::add_columns(acc, t0, [&] { return slot[row]; }, [&] {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&tmem_empty[buf]);
-        });
-        if (++buf == kBufs) buf = 0, phase ^= 1u;
-        continue;
-      }
       uint32_t v[2][16];
       auto load = [&](int c, uint32_t(&r)[16]) {
         if constexpr (kFragments) fp8::tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>(c & 1) * 16) << 16) + (c >> 1) * 32, r);
         else fp8::tmem_ld_x16(t0 + c * 16, r);
       };
       load(0, v[0]);
-      const float mine = kSwap && kRows ? slot[TM + row] : 1.0f;
+      const float mine = kSwap ? (kRows ? slot[TM + row] : 1.0f) : (kFragments ? 1.0f : slot[row]);
       float lo_hi[4];
       float2 cs[2][4];  // column scales, loaded two steps ahead
       const float2* sb = reinterpret_cast<const float2*>(slot + TM) + (lane & 3);
@@ -318,6 +312,9 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
             for (int q = 0; q < 4; ++q)
               acc[c * 16 + j + q] = fmaf(kRows ? f[q] * mine : f[q], __uint_as_float(r[j + q]), acc[c * 16 + j + q]);
           }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(mine, __uint_as_float(r[j]), acc[c * 16 + j]);
         }
       }
       if constexpr (kSwap) {
