@@ -147,6 +147,29 @@ def test_no_gradient_is_refused():
 # ---------------------------------------------------------------- decoder layer
 
 
+def test_no_gradient_of_tables_and_8_bit_operands_is_refused():
+    """Operands without a gradient that require one: refused, not dropped from the graph."""
+    torch_ops.load()
+    q = torch.zeros(4, 2, 8)
+    pos, table = torch.zeros(4, dtype=torch.int64), torch.zeros(16, 8)
+    wq, s = torch.zeros(16, 128).to(torch.float8_e4m3fn), torch.ones(1, 1)
+    x, xs = torch.zeros(4, 128), torch.ones(4, 1)
+    grad_table, grad_w = table.clone().requires_grad_(), wq.clone().requires_grad_()
+    a = torch.zeros(4, 128).to(torch.float8_e4m3fn)
+    calls = [
+        lambda: torch_ops.rotary(q, q, pos, grad_table),
+        lambda: torch_ops.rotary(q.clone().requires_grad_(), q, pos, grad_table),
+        lambda: torch_ops.rotary_(q, q, pos, grad_table),
+        lambda: torch_ops.linear_fp8(x, grad_w, s),
+        lambda: torch_ops.linear_fp8_out(x, grad_w, s, torch.zeros(4, 16)),
+        lambda: torch_ops.gemm_fp8(a, xs, grad_w, s),
+        lambda: torch_ops.gemm_fp8(a.clone().requires_grad_(), xs, wq, s),
+    ]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            call()
+
+
 def test_rotary_heads_of_a_shard():
     from zcutlass_b200 import tp
 

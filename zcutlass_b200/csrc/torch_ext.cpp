@@ -555,6 +555,8 @@ at::Tensor linear_fp8_train_autograd(const at::Tensor& x, const at::Tensor& w, c
   return LinearFp8::apply(x, w, bias, wants_grad(x), wants_grad(w), wants_grad(b));
 }
 
+constexpr char kTableGradient[] = "the table of rotary positions has no gradient: detach it";
+
 class Rotary : public torch::autograd::Function<Rotary> {
  public:
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
@@ -571,6 +573,7 @@ class Rotary : public torch::autograd::Function<Rotary> {
 
 std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                                                    const at::Tensor& table, bool interleaved, bool inverse) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(table), kTableGradient);
   if (!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k))) {
     const at::AutoDispatchBelowADInplaceOrView guard;
     return rotary_op(q, k, positions, table, interleaved, inverse);
@@ -601,21 +604,21 @@ std::vector<at::Tensor> quantize_fp8_autograd(const at::Tensor& x, std::string_v
 
 at::Tensor gemm_fp8_autograd(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale,
                              const std::optional<at::Tensor>& bias, std::optional<at::ScalarType> out_dtype) {
-  check_no_gradient("gemm_fp8", a_scale, b_scale, bias.value_or(at::Tensor()));
+  check_no_gradient("gemm_fp8", a, b, a_scale, b_scale, bias.value_or(at::Tensor()));
   const at::AutoDispatchBelowADInplaceOrView guard;
   return gemm_fp8_op(a, a_scale, b, b_scale, bias, out_dtype);
 }
 
 at::Tensor linear_fp8_autograd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
                                const std::optional<at::Tensor>& bias) {
-  check_no_gradient("linear_fp8", x, w_scale, bias.value_or(at::Tensor()));
+  check_no_gradient("linear_fp8", x, w, w_scale, bias.value_or(at::Tensor()));
   const at::AutoDispatchBelowADInplaceOrView guard;
   return linear_fp8_op(x, w, w_scale, bias);
 }
 
 void linear_fp8_out_autograd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
                              const std::optional<at::Tensor>& bias, at::Tensor out) {
-  check_no_gradient("linear_fp8_out", x, w_scale, bias.value_or(at::Tensor()), out);
+  check_no_gradient("linear_fp8_out", x, w, w_scale, bias.value_or(at::Tensor()), out);
   const at::AutoDispatchBelowADInplaceOrView guard;
   linear_fp8_out_op(x, w, w_scale, bias, out);
   out.unsafeGetTensorImpl()->bump_version();
@@ -625,6 +628,7 @@ void rotary_inplace_autograd(at::Tensor q, at::Tensor k, const at::Tensor& posit
                              bool interleaved, bool inverse) {
   TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k)),
               "rotary_ has no gradient: use rotary, or call it under torch.no_grad()");
+  TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(table), kTableGradient);
   const at::AutoDispatchBelowADInplaceOrView guard;
   rotary_inplace_op(q, k, positions, table, interleaved, inverse);
   // Saved for a backward pass elsewhere, the old values are gone: let autograd see it.
