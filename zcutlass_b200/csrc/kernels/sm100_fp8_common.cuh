@@ -126,7 +126,7 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return d;
 }
 
-// The same for registers already waited for.
+// Registers of a load that has been waited for: no use of them moves above this point.
 __device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; i += 8)

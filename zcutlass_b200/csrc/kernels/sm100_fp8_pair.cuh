@@ -9,7 +9,10 @@
 // read the buffer and add it, scaled, into 128 32-bit accumulators per thread,
 // while the MMAs of the next block fill the other buffer.
 //
-// What bounds it: at full rate a block takes the tensor pipe 512 cycles (531
+// What bounds it: power for long products (8192 x 28672 x 4096 takes 615 us on
+// zeros; on random bits 770-800 in a burst and 884 sustained, at 990 W and 1.4
+// GHz with the power cap active), else a buffer's turnaround. At full rate a
+// block takes the tensor pipe 512 cycles (531
 // measured), TMEM reads and 32-bit fma 260-350. A buffer's turnaround (MMAs,
 // commit, read, arrival at the leader) must fit two blocks' time, so nothing
 // slow may sit on it:
@@ -21,6 +24,9 @@
 //    idle warps, one per TMEM buffer, put each block's scales in shared memory
 //    and complete the buffer's `tmem_full` barrier together with the commit;
 //  - the arrival at the leader's `tmem_empty` is not a cluster-wide release.
+//
+// Measured (random bits, 20 in a row): 8192 x 9472 x 4096 266 us, 2387 TFLOP/s;
+// with a scale per row of B 348 us, 1825 TFLOP/s.
 //
 // With 128 x 128 weight scales the factor is one product per thread and block.
 // With a scale per row of B (kRows) TMEM is read as 16 x 8 fragments, in which

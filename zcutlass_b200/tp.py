@@ -475,9 +475,9 @@ class TPDecoderLinears:
         self.sp_gather = "copy"
 
     def quantize_fp8(self) -> None:
-        """Replaces the four weights by 8-bit ones (Fp8Weight), a quarter to a
-        half of the layer's memory traffic at decode and twice the tensor rate
-        at prefill. The 16-bit weights are dropped; idempotent."""
+        """Replaces the four weights by 8-bit ones (Fp8Weight), half the
+        bytes that a decode step reads. The 16-bit weights are dropped;
+        idempotent."""
         for linear in (self.qkv, self.o_proj, self.gate_up, self.down):
             if not isinstance(linear.weight, Fp8Weight):
                 linear.weight = Fp8Weight(linear.weight)
