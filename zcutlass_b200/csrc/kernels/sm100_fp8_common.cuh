@@ -127,9 +127,10 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 // Registers of a load that has been waited for: no use of them moves above this point.
-__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
+template <int N>
+__device__ __forceinline__ void after_wait(uint32_t (&r)[N]) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 8)
+  for (int i = 0; i < N; i += 8)
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 

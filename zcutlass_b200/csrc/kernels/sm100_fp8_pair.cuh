@@ -12,10 +12,9 @@
 // What bounds it: power for long products (8192 x 28672 x 4096 takes 615 us on
 // zeros; on random bits 770-800 in a burst and 884 sustained, at 990 W and 1.4
 // GHz with the power cap active), else a buffer's turnaround. At full rate a
-// block takes the tensor pipe 512 cycles (531
-// measured), TMEM reads and 32-bit fma 260-350. A buffer's turnaround (MMAs,
-// commit, read, arrival at the leader) must fit two blocks' time, so nothing
-// slow may sit on it:
+// block takes the tensor pipe 512 cycles (531 measured), TMEM reads and 32-bit
+// fma 343 by themselves. A buffer's turnaround (MMAs, commit, read, arrival at the
+// leader) must fit two blocks' time, so nothing slow may sit on it:
 //  - the warp that issues MMAs walks its loop as a whole, with its state in
 //    uniform registers and one lane issuing (per-lane descriptors alone halved
 //    the MMA rate: the accumulation warps leave few issue slots);
@@ -26,12 +25,16 @@
 //  - the arrival at the leader's `tmem_empty` is not a cluster-wide release.
 //
 // Measured (random bits, 20 in a row): 8192 x 9472 x 4096 266 us, 2387 TFLOP/s;
-// with a scale per row of B 348 us, 1825 TFLOP/s.
+// with a scale per row of B 344 us, 1848 TFLOP/s.
 //
 // With 128 x 128 weight scales the factor is one product per thread and block.
 // With a scale per row of B (kRows) TMEM is read as 16 x 8 fragments, in which
 // a thread meets only 32 of the 128 columns: a quarter of the shared-memory
-// reads that a row per thread would need.
+// reads that a row per thread would need. Such loads bring 16 of 32 lanes at a
+// time; they bound this variant. Cycles per block, the accumulation alone: a row
+// per thread with one scale 343, fragments 720 (565 with the scales in
+// registers), a row per thread with scales from shared memory 764, part of the
+// columns each way 748 to 804.
 //
 // Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocation and, in the
 // leader, MMA issue, warps 2-3 scales; warps 4-11 accumulate, then write the
@@ -377,26 +380,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (!kRows) {
           fp8::add_columns(acc, t0, [&] { return slot[quarter * 32 + lane] * slot[kHalf + half]; }, read_done);
         } else {
-          uint32_t v[2][16];
-          fp8::tmem_ld_16x256b_x4(t0, v[0]);
+          // 32 columns of 16 rows per load: v[0], v[1] the two halves of the rows in one column group, v[2], v[3]
+          // in the next. Four loads are in flight at a time (one ahead: 1 % slower).
+          uint32_t v[4][16];
+          const auto load = [&](int g) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              fp8::tmem_ld_16x256b_x4(t0 + (static_cast<uint32_t>(h * 16) << 16) + g * 32, v[2 * (g & 1) + h]);
+          };
+          const auto landed = [&] {
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fp8::after_wait(v[j]);
+          };
+          load(0);
+          load(1);
           float sa[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) sa[j] = slot[quarter * 32 + j * 8 + (lane >> 2)];
           const float2* sb = reinterpret_cast<const float2*>(slot + kHalf + half * kHalf) + (lane & 3);
-          float2 cs[2][4];  // column scales, loaded two steps ahead
-          fp8::load_column_scales(cs[0], sb);
+          float2 cs[2][4];  // column scales of two groups
+          const auto add = [&](int g) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {  // 32 columns of 16 rows per step: (c / 2, c % 2)
-            uint32_t(&r)[16] = v[c & 1];
-            if (c % 2 == 0 && c < 6) fp8::load_column_scales(cs[(c / 2 + 1) & 1], sb + (c / 2 + 1) * 16);
-            fp8::tmem_ld_wait_x16(r);
-            if (c + 1 < 8) {
-              fp8::tmem_ld_16x256b_x4(t0 + ((static_cast<uint32_t>((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, v[(c + 1) & 1]);
-            } else {
-              read_done();  // of the slot, too: the last column scales were used in the step before
-            }
-            fp8::add_fragments(acc + (c >> 1) * 32 + (c & 1) * 16, r, cs[(c / 2) & 1], sa[2 * (c & 1)], sa[2 * (c & 1) + 1]);
-          }
+            for (int h = 0; h < 2; ++h)
+              fp8::add_fragments(acc + g * 32 + h * 16, v[2 * (g & 1) + h], cs[g & 1], sa[2 * h], sa[2 * h + 1]);
+          };
+          fp8::load_column_scales(cs[0], sb);
+          fp8::load_column_scales(cs[1], sb + 16);
+          landed();
+          add(0);
+          load(2);
+          fp8::load_column_scales(cs[0], sb + 32);
+          add(1);
+          load(3);
+          fp8::load_column_scales(cs[1], sb + 48);
+          landed();
+          read_done();  // of the slot, too
+          add(2);
+          add(3);
         }
       }
       if (!ok) break;
