@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
     if (p.splits == 1) {
 #pragma unroll 4
       for (int mi = first; mi < rows; mi += per) put(mi, *reinterpret_cast<const float4*>(red + red_at<kSwap>(mi, g)));
-    } else if (first < per) {
+    } else if (first < per && n < p.n) {  // every load below feeds a store: none may be left in flight
 #pragma unroll 2
       for (int mi = first; mi < rows; mi += per) {
         const uint32_t off = static_cast<uint32_t>(red_at<kSwap>(mi, g) * 4);
@@ -401,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
     }
   }
   __syncwarp();
-  // No CTA leaves while a peer may still read its partial tile. The reads are done (their sums were used) and
-  // nothing is handed over, so the arrival need not wait for the stores to D.
+  // No CTA leaves while a peer may still read its partial tile. Each thread's reads are done, since it has
+  // stored their sums, and nothing is handed over, so the arrival need not wait for the stores to D.
   if (p.splits > 1) fp8::cluster_sync_relaxed();
   if (warp == 1) {
     tc_fence_after_sync();
