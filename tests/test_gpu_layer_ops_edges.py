@@ -32,3 +32,48 @@ def test_split_product_with_groups_beyond_the_last_column(cuda_device, monkeypat
         R.check_product(d[0], *R.product(a, sa, b, sb), 2100)
         assert all(torch.equal(x, d[0]) for x in d)
     assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("layout", ["blocks", "rows"])
+@pytest.mark.parametrize("m", [1, 40, 200, 2400])
+def test_scales_that_the_kernel_before_has_just_written(cuda_device, m, layout):
+    """Two inputs in turn through recycled buffers, nothing waited for in between."""
+    w = [rand(1100, 1500, seed=s) * 2.0 ** (5 * s) for s in (0, 1)]
+    x = [rand(m, 1500, seed=s + 2) * 2.0 ** (7 * s) for s in (0, 1)]
+
+    def step(i):
+        b, sb = torch_ops.quantize_fp8(w[i], layout=layout)
+        a, sa = torch_ops.quantize_fp8(x[i])
+        return torch_ops.gemm_fp8(a, sa, b, sb, out_dtype=F32)
+
+    want = []
+    for i in (0, 1):
+        want.append(step(i))
+        torch.cuda.synchronize()
+    wrong = torch.zeros((), device="cuda", dtype=torch.int64)
+    for t in range(40):
+        wrong += (step(t % 2) != want[t % 2]).sum()
+    assert wrong.item() == 0
+
+
+@pytest.mark.parametrize("rot", [64, 6])
+def test_rotary_table_that_the_kernel_before_has_just_written(cuda_device, rot):
+    q, k = rand(500, 4, 64, seed=1), rand(500, 2, 64, seed=2)
+    pos = torch.arange(500, device="cuda") % 300
+    b, sb = torch_ops.quantize_fp8(rand(rot, 256, seed=3), layout="rows")
+    a = [torch_ops.quantize_fp8(rand(300, 256, seed=4 + i)) for i in (0, 1)]
+
+    def step(i):
+        table = torch_ops.gemm_fp8(*a[i], b, sb, out_dtype=F32)
+        return torch_ops.rotary(q, k, pos, table)
+
+    want = []
+    for i in (0, 1):
+        want.append(step(i))
+        torch.cuda.synchronize()
+        R.check_rotated(want[i][0], q, pos, torch_ops.gemm_fp8(*a[i], b, sb, out_dtype=F32), False)
+    wrong = torch.zeros((), device="cuda", dtype=torch.int64)
+    for t in range(100):
+        got = step(t % 2)
+        wrong += sum((x != y).sum() for x, y in zip(got, want[t % 2]))
+    assert wrong.item() == 0

@@ -136,14 +136,14 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
     if constexpr (kPairs % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < kPairs; i += 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(row + i));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(row + half + i));
+        const float4 a = ld_written(reinterpret_cast<const float4*>(row + i));
+        const float4 b = ld_written(reinterpret_cast<const float4*>(row + half + i));
         c[i] = a.x, c[i + 1] = a.y, c[i + 2] = a.z, c[i + 3] = a.w;
         s[i] = b.x, s[i + 1] = b.y, s[i + 2] = b.z, s[i + 3] = b.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) c[i] = __ldg(row + i), s[i] = __ldg(row + half + i);
+      for (int i = 0; i < kPairs; ++i) c[i] = ld_written(row + i), s[i] = ld_written(row + half + i);
     }
     if (p.inverse) {
 #pragma unroll

@@ -315,16 +315,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < kHalf / 32; ++j) {
             const int64_t row = m0 + j * 32 + lane;
-            a[j] = row < p.m ? __ldg(sa + row * p.a_scale_row) : 0.0f;
+            a[j] = row < p.m ? ld_written(sa + row * p.a_scale_row) : 0.0f;
           }
           if constexpr (kRows) {
 #pragma unroll
             for (int j = 0; j < kBlock / 32; ++j) {
               const int64_t col = n0 + j * 32 + lane;
-              b[j] = col < p.n ? __ldg(sb + col * p.b_scale_row) : 0.0f;
+              b[j] = col < p.n ? ld_written(sb + col * p.b_scale_row) : 0.0f;
             }
           } else {
-            b[0] = lane < 2 && n0 + lane * kHalf < p.n ? __ldg(sb + (n0 / kHalf + lane) * p.b_scale_row) : 0.0f;
+            b[0] = lane < 2 && n0 + lane * kHalf < p.n ? ld_written(sb + (n0 / kHalf + lane) * p.b_scale_row) : 0.0f;
           }
           if (i >= kBufs) ok = fp8::wait(&tmem_full[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrScaleTmemFull);
           ok = __all_sync(0xffffffffu, ok);

@@ -226,16 +226,16 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
 #pragma unroll
       for (int j = 0; j < kA; ++j) {
         const int r = j * 32 + lane;
-        a[j] = r < TM && m0 + r < p.m ? __ldg(sa + (m0 + r) * p.a_scale_row) : 0.0f;
+        a[j] = r < TM && m0 + r < p.m ? ld_written(sa + (m0 + r) * p.a_scale_row) : 0.0f;
       }
       if constexpr (kRows) {
 #pragma unroll
         for (int j = 0; j < kBlockN / 32; ++j) {
           const int r = n0 + j * 32 + lane;
-          b[j] = r < p.n ? __ldg(sb + r * p.b_scale_row) : 0.0f;
+          b[j] = r < p.n ? ld_written(sb + r * p.b_scale_row) : 0.0f;
         }
       } else {
-        b[0] = __ldg(sb + (n0 / kBlockN) * p.b_scale_row);
+        b[0] = ld_written(sb + (n0 / kBlockN) * p.b_scale_row);
       }
       if (i >= kBufs) ok = fp8::wait(&tmem_full[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrScaleTmemFull);
       ok = __all_sync(0xffffffffu, ok);
