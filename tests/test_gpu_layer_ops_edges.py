@@ -77,3 +77,26 @@ def test_rotary_table_that_the_kernel_before_has_just_written(cuda_device, rot):
         got = step(t % 2)
         wrong += sum((x != y).sum() for x, y in zip(got, want[t % 2]))
     assert wrong.item() == 0
+
+
+@pytest.mark.parametrize("layout", ["blocks", "rows"])
+def test_pair_product_hands_buffers_and_scales_back(cuda_device, monkeypatch, layout):
+    """Many k blocks, each with scales far from its neighbours' (a block scaled by another's is off by 2^5 or
+    more), several tiles per pair, beside memory traffic on another stream."""
+    monkeypatch.setenv("ZCUTLASS_FORCE_KERNEL", "fp8_pair")
+    m, n, k = 2300, 2500, 4224
+    swing = (2.0 ** (5 * (torch.arange(33, device="cuda") % 7))).repeat_interleave(128)
+    a, sa = torch_ops.quantize_fp8(rand(m, k, seed=1) * swing)
+    b, sb = torch_ops.quantize_fp8(rand(n, k, seed=2) / swing, layout=layout)
+    want = torch_ops.gemm_fp8(a, sa, b, sb, out_dtype=F32)
+    R.check_product(want, *R.product(a, sa, b, sb), k)
+    torch.cuda.synchronize()
+    noise = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+    wrong = torch.zeros((), device="cuda", dtype=torch.int64)
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            noise.add_(1)
+        wrong += (torch_ops.gemm_fp8(a, sa, b, sb, out_dtype=F32) != want).sum()
+    torch.cuda.synchronize()
+    assert wrong.item() == 0 and _native.device_error() == 0

@@ -21,8 +21,10 @@
 //  - scales never pass through the accumulation warps' registers as loads in
 //    flight (a wait loop holds them up until the load returns): two otherwise
 //    idle warps, one per TMEM buffer, put each block's scales in shared memory
-//    and complete the buffer's `tmem_full` barrier together with the commit;
-//  - the arrival at the leader's `tmem_empty` is not a cluster-wide release.
+//    and complete the buffer's `tmem_full` barrier together with the commit.
+//    The scales are handed back on a barrier of this CTA, `read`;
+//  - the arrival at the leader's `tmem_empty` hands back TMEM alone, so it is
+//    not a release of memory to the cluster.
 //
 // Measured (random bits, 20 in a row): 8192 x 9472 x 4096 266 us, 2387 TFLOP/s;
 // with a scale per row of B 344 us, 1848 TFLOP/s.
@@ -74,7 +76,6 @@ constexpr int kThreads = 384;
 constexpr int kAuxThreads = 128;
 constexpr int kAccWarps = 8;
 constexpr int kBufs = 2;
-constexpr int kSlots = 4;     // blocks whose scales are in shared memory
 constexpr uint32_t kTmemCols = 512;
 
 template <bool kRows>
@@ -86,8 +87,8 @@ struct Smem {
   static constexpr int kOutWarp = 8192;  // per accumulation warp: four chunks of 32 rows x 64 bytes
   static constexpr int kSlotFloats = kHalf + (kRows ? kBlock : 8);  // row scales, column (block) scales
   static constexpr int kScaleOff = kOutOff + kAccWarps * kOutWarp;
-  static constexpr int kBarOff = kScaleOff + kSlots * kSlotFloats * 4;
-  static constexpr int kNumBars = 2 * kStages + 2 * kBufs + 1;
+  static constexpr int kBarOff = kScaleOff + kBufs * kSlotFloats * 4;  // the scales of each TMEM buffer's block
+  static constexpr int kNumBars = 2 * kStages + 3 * kBufs + 1;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kDynamicBytes = kMiscOff + 8;
   static_assert(kDynamicBytes <= 232448, "shared memory budget exceeded");
@@ -98,7 +99,7 @@ enum : int {
   kErrMmaFull = (34 << 4) | 2,
   kErrMmaTmemEmpty = (34 << 4) | 3,
   kErrAccTmemFull = (34 << 4) | 4,
-  kErrScaleTmemFull = (34 << 4) | 5,
+  kErrScaleRead = (34 << 4) | 5,
   kErrAlignment = (34 << 4) | 6,
 };
 
@@ -177,7 +178,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + kStages;
   uint64_t* tmem_full = empty + kStages;
   uint64_t* tmem_empty = tmem_full + kBufs;  // used in the leader
-  uint64_t* drain = tmem_empty + kBufs;
+  uint64_t* read = tmem_empty + kBufs;  // this CTA's warps have read the buffer and its scales
+  uint64_t* drain = read + kBufs;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
   float* const slots = reinterpret_cast<float*>(smem + L::kScaleOff);
@@ -199,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int b = 0; b < kBufs; ++b) {
       mbar_init(&tmem_full[b], 2);  // the commit and the scales
       mbar_init(&tmem_empty[b], 2 * kAccWarps);
+      mbar_init(&read[b], kAccWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int tile = pair; ok && tile < p.total_tiles; tile += npairs) {
           for (int kb = 0; kb < p.num_kb; ++kb) {
             ok = fp8::wait(&full[s], phase, ctx, kErrMmaFull);
-            ok = ok && fp8::wait(&tmem_empty[buf], buf_phase, ctx, kErrMmaTmemEmpty);
+            ok = ok && fp8::wait_read(&tmem_empty[buf], buf_phase, ctx, kErrMmaTmemEmpty);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after_sync();
@@ -297,8 +300,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     } else {
       // ------------------------------------------------------------ scales (both CTAs)
-      // Warp 2 + b serves the blocks of TMEM buffer b. Slot i % 4 is rewritten once phase i - 2 of the buffer
-      // is complete: its MMAs were issued after every warp had read block i - 4.
+      // Warp 2 + b serves the blocks of TMEM buffer b: block i's scales go where block i - 2's were once every
+      // warp of this CTA has read those. So the buffer's `tmem_full` phase of block i - 2 is complete, too.
       const uint32_t buf = static_cast<uint32_t>(warp - 2);
       uint32_t i = 0;  // blocks so far, both buffers'
       bool ok = true;
@@ -326,10 +329,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             b[0] = lane < 2 && n0 + lane * kHalf < p.n ? ld_written(sb + (n0 / kHalf + lane) * p.b_scale_row) : 0.0f;
           }
-          if (i >= kBufs) ok = fp8::wait(&tmem_full[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrScaleTmemFull);
+          if (i >= kBufs) ok = fp8::wait(&read[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrScaleRead);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          float* slot = slots + (i % kSlots) * L::kSlotFloats;
+          float* slot = slots + buf * L::kSlotFloats;
 #pragma unroll
           for (int j = 0; j < kHalf / 32; ++j) slot[j * 32 + lane] = a[j];
           if constexpr (kRows) {
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int kb = 0; kb < p.num_kb; ++kb, ++i) {
         const uint32_t buf = i % kBufs;
-        const float* slot = slots + (i % kSlots) * L::kSlotFloats;
+        const float* slot = slots + buf * L::kSlotFloats;
         ok = fp8::wait(&tmem_full[buf], (i / kBufs) & 1u, ctx, kErrAccTmemFull);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -375,7 +378,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const auto read_done = [&] {
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
+          if (lane == 0) {
+            fp8::arrive_read(map_shared_rank(smem_addr(&tmem_empty[buf]), 0));
+            mbar_arrive(&read[buf]);
+          }
         };
         if constexpr (!kRows) {
           fp8::add_columns(acc, t0, [&] { return slot[quarter * 32 + lane] * slot[kHalf + half]; }, read_done);
@@ -415,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           load(3);
           fp8::load_column_scales(cs[1], sb + 48);
           landed();
-          read_done();  // of the slot, too
+          read_done();
           add(2);
           add(3);
         }
