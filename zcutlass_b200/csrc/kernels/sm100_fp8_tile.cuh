@@ -52,7 +52,6 @@ constexpr int kThreads = 256;
 constexpr int kAccThreads = 128;
 constexpr int kMaxSplits = 8;
 constexpr int kBufs = 4;   // TMEM buffers
-constexpr int kSlots = 8;  // blocks whose scales are in shared memory
 
 template <bool kSwap, int TM, bool kRows, int STAGES, int KSUB>
 struct Smem {
@@ -66,7 +65,7 @@ struct Smem {
   static constexpr int kRing = STAGES * kStageBytes > kRedBytes ? STAGES * kStageBytes : kRedBytes;
   static constexpr int kSlotFloats = TM + (kRows ? kBlockN : 0);
   static constexpr int kScaleOff = kRing;
-  static constexpr int kBarOff = kScaleOff + kSlots * kSlotFloats * 4;
+  static constexpr int kBarOff = kScaleOff + kBufs * kSlotFloats * 4;  // the scales of each TMEM buffer's block
   static constexpr int kNumBars = 2 * STAGES + 2 * kBufs + 1;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kDynamicBytes = kMiscOff + 16 + 1024;
@@ -79,7 +78,7 @@ enum : int {
   kErrMmaFull = (33 << 4) | 2,
   kErrMmaTmemEmpty = (33 << 4) | 3,
   kErrAccTmemFull = (33 << 4) | 4,
-  kErrScaleTmemFull = (33 << 4) | 5,
+  kErrScaleRead = (33 << 4) | 5,
 };
 
 // Partial tile element (m, 4 g): rows rotate their 16-byte units where a thread writes a whole row.
@@ -214,8 +213,8 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
     }
     __syncwarp();
   } else if (warp < 4) {
-    // Scales: warp 2 + q serves the blocks of parity q. Slot i % 8 is rewritten once phase i - 4 of its
-    // buffer is complete: its MMAs were issued after every warp had read block i - 8.
+    // Scales: warp 2 + q serves the blocks of parity q. Block i's go where block i - 4's were once every warp has
+    // read those and the TMEM buffer, so the buffer's `tmem_full` phase of block i - 4 is complete, too.
     bool ok = true;
     for (int kb = kb0 + warp - 2; ok && kb < kb1; kb += 2) {
       const uint32_t i = static_cast<uint32_t>(kb - kb0), buf = i % kBufs;
@@ -237,10 +236,10 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
       } else {
         b[0] = ld_written(sb + (n0 / kBlockN) * p.b_scale_row);
       }
-      if (i >= kBufs) ok = fp8::wait(&tmem_full[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrScaleTmemFull);
+      if (i >= kBufs) ok = fp8::wait(&tmem_empty[buf], ((i / kBufs) & 1u) ^ 1u, ctx, kErrScaleRead);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      float* slot = slots + (i % kSlots) * L::kSlotFloats;
+      float* slot = slots + buf * L::kSlotFloats;
 #pragma unroll
       for (int j = 0; j < kA; ++j)
         if (j * 32 + lane < TM) slot[j * 32 + lane] = kRows ? a[j] : a[j] * b[0];
@@ -265,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, kSwap ? 2 : 1)
     uint32_t buf = 0, phase = 0;
 #pragma unroll 1
     for (int kb = kb0; kb < kb1; ++kb) {
-      const float* slot = slots + ((kb - kb0) % kSlots) * L::kSlotFloats;
+      const float* slot = slots + buf * L::kSlotFloats;
       ok = __all_sync(0xffffffffu, fp8::wait(&tmem_full[buf], phase, ctx, kErrAccTmemFull));
       if (!ok) break;
       tc_fence_after_sync();
