@@ -1,0 +1,56 @@
+"""Host side of the 8-bit linears and rotary positions, without a GPU: calls that would lose something
+without a word are refused, and refusals say what they refuse."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from zcutlass_b200 import torch_ops
+
+E4M3 = torch.float8_e4m3fn
+
+
+def operands():
+    torch_ops.load()
+    return dict(x=torch.ones(4, 128), w=torch.ones(16, 128), bias=torch.ones(16), s=torch.ones(1, 1), xs=torch.ones(4, 1),
+                q=torch.ones(4, 2, 8), pos=torch.zeros(4, dtype=torch.int64), table=torch.zeros(16, 8), out=torch.ones(4, 16))
+
+
+# (operator, operand that carries the derivative, call)
+CALLS = [
+    ("quantize_fp8", "x", lambda o: torch_ops.quantize_fp8(o["x"])),
+    ("gemm_fp8", "xs", lambda o: torch_ops.gemm_fp8(o["x"].detach().to(E4M3), o["xs"], o["w"].to(E4M3), o["s"])),
+    ("gemm_fp8", "s", lambda o: torch_ops.gemm_fp8(o["x"].to(E4M3), o["xs"], o["w"].to(E4M3), o["s"])),
+    ("linear_fp8", "x", lambda o: torch_ops.linear_fp8(o["x"], o["w"].to(E4M3), o["s"])),
+    ("linear_fp8", "bias", lambda o: torch_ops.linear_fp8(o["x"], o["w"].to(E4M3), o["s"], o["bias"])),
+    ("linear_fp8_out", "x", lambda o: torch_ops.linear_fp8_out(o["x"], o["w"].to(E4M3), o["s"], o["out"])),
+    ("linear_fp8_out", "out", lambda o: torch_ops.linear_fp8_out(o["x"], o["w"].to(E4M3), o["s"], o["out"])),
+    ("linear_fp8_train", "x", lambda o: torch_ops.linear_fp8_train(o["x"], o["w"])),
+    ("linear_fp8_train", "w", lambda o: torch_ops.linear_fp8_train(o["x"], o["w"], o["bias"])),
+    ("linear_fp8_train", "bias", lambda o: torch_ops.linear_fp8_train(o["x"], o["w"], o["bias"])),
+    ("rotary", "q", lambda o: torch_ops.rotary(o["q"], o["q"].detach() * 1, o["pos"], o["table"])),
+    ("rotary", "table", lambda o: torch_ops.rotary(o["q"], o["q"], o["pos"], o["table"])),
+    ("rotary_", "q", lambda o: torch_ops.rotary_(o["q"], torch.ones(4, 2, 8), o["pos"], o["table"])),
+]
+
+
+@pytest.mark.parametrize("grad", [True, False], ids=["grad", "no_grad"])
+@pytest.mark.parametrize("name,operand,call", CALLS, ids=lambda v: v if isinstance(v, str) else "")
+def test_forward_mode_is_refused(name, operand, call, grad):
+    """A tangent is refused, not dropped: in dual numbers and in torch.func.jvp, with and without no_grad (which
+    does not switch forward mode off)."""
+    o = operands()
+    t = o[operand]
+    match = f"{name} has no forward-mode derivative"
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        o[operand] = forward_ad.make_dual(t, torch.ones_like(t))
+        with pytest.raises(RuntimeError, match=match):
+            call(o)
+    if grad:
+        with pytest.raises(RuntimeError, match=match):
+            torch.func.jvp(lambda v: call({**operands(), operand: v}), (t,), (torch.ones_like(t),))
+    o[operand] = t  # without a tangent, the call goes on to its own checks
+    with pytest.raises(RuntimeError, match="CUDA|cuda"):
+        call(o)

@@ -495,6 +495,13 @@ using torch::autograd::variable_list;
 
 bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// Forward-mode derivatives: a tensor with a tangent need not require a gradient, and the kernels run below
+// autograd, so its tangent would be dropped (in place: kept beside values it no longer belongs to).
+template <typename... T>
+void check_no_tangent(const char* name, const T&... t) {
+  TORCH_CHECK(!((t.defined() && t._fw_grad(0).defined()) || ...), name, " has no forward-mode derivative");
+}
+
 // While the current stream is being captured: refuses a leaf whose gradient accumulator was made on another
 // stream and is still alive (an eager graph of the same leaf is). The backward pass would wait for that
 // stream, which ends the capture, or the process.
@@ -511,6 +518,7 @@ void check_capture(const at::Tensor& leaf) {
 
 template <typename... T>
 void check_no_gradient(const char* name, const T&... t) {
+  check_no_tangent(name, t...);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(t) || ...), name,
               " has no gradient: use linear_fp8_train, or call it under torch.no_grad()");
 }
@@ -545,6 +553,7 @@ class LinearFp8 : public torch::autograd::Function<LinearFp8> {
 
 at::Tensor linear_fp8_train_autograd(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias) {
   const at::Tensor b = bias.value_or(at::Tensor());
+  check_no_tangent("linear_fp8_train", x, w, b);
   if (!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || wants_grad(b))) {
     const at::AutoDispatchBelowADInplaceOrView guard;
     return linear_fp8_train_op(x, w, bias);
@@ -573,6 +582,7 @@ class Rotary : public torch::autograd::Function<Rotary> {
 
 std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                                                    const at::Tensor& table, bool interleaved, bool inverse) {
+  check_no_tangent("rotary", q, k, table);
   TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(table), kTableGradient);
   if (!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k))) {
     const at::AutoDispatchBelowADInplaceOrView guard;
@@ -626,6 +636,7 @@ void linear_fp8_out_autograd(const at::Tensor& x, const at::Tensor& w, const at:
 
 void rotary_inplace_autograd(at::Tensor q, at::Tensor k, const at::Tensor& positions, const at::Tensor& table,
                              bool interleaved, bool inverse) {
+  check_no_tangent("rotary_", q, k, table);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k)),
               "rotary_ has no gradient: use rotary, or call it under torch.no_grad()");
   TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(table), kTableGradient);
