@@ -54,3 +54,10 @@ def test_forward_mode_is_refused(name, operand, call, grad):
     o[operand] = t  # without a tangent, the call goes on to its own checks
     with pytest.raises(RuntimeError, match="CUDA|cuda"):
         call(o)
+
+
+def test_rotary_on_cpu_tensors_says_so():
+    o = operands()
+    for call in (torch_ops.rotary, torch_ops.rotary_):
+        with pytest.raises(RuntimeError, match="q must be a rank-3 CUDA tensor"):
+            call(o["q"], o["q"].clone(), o["pos"], o["table"])

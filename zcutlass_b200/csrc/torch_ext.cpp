@@ -431,6 +431,7 @@ at::Tensor linear_fp8_train_op(const at::Tensor& x, const at::Tensor& w, const s
 
 // ---------------------------------------------------------------- rotary positions
 
+// The checks of q and k, before anything is allocated or a device is made current.
 void check_heads(const at::Tensor& t, const char* name, const at::Tensor& q) {
   TORCH_CHECK(t.is_cuda() && t.dim() == 3, name, " must be a rank-3 CUDA tensor [tokens, heads, head_dim]");
   (void)float_code(t, name);
@@ -442,8 +443,6 @@ void check_heads(const at::Tensor& t, const char* name, const at::Tensor& q) {
 
 void run_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_out, const at::Tensor& k_out,
                 const at::Tensor& positions, const at::Tensor& table, bool interleaved, bool inverse) {
-  check_heads(q, "q", q);
-  check_heads(k, "k", q);
   TORCH_CHECK(positions.device() == q.device() && table.device() == q.device(),
               "positions and table must be on the device of q and k");
   TORCH_CHECK(positions.dim() == 1 && positions.is_contiguous() && positions.size(0) == q.size(0),
@@ -472,8 +471,9 @@ void run_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_ou
 
 std::tuple<at::Tensor, at::Tensor> rotary_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                                              const at::Tensor& table, bool interleaved, bool inverse) {
+  check_heads(q, "q", q);
+  check_heads(k, "k", q);
   const c10::cuda::CUDAGuard guard(q.device());
-  TORCH_CHECK(q.is_cuda() && k.is_cuda(), "q and k must be CUDA tensors");
   at::Tensor q_out = empty_like_device(q.sizes(), q.scalar_type(), q), k_out = empty_like_device(k.sizes(), k.scalar_type(), k);
   run_rotary(q, k, q_out, k_out, positions, table, interleaved, inverse);
   return {q_out, k_out};
@@ -481,6 +481,8 @@ std::tuple<at::Tensor, at::Tensor> rotary_op(const at::Tensor& q, const at::Tens
 
 void rotary_inplace_op(at::Tensor q, at::Tensor k, const at::Tensor& positions, const at::Tensor& table,
                        bool interleaved, bool inverse) {
+  check_heads(q, "q", q);
+  check_heads(k, "k", q);
   at::assert_no_internal_overlap(q);
   at::assert_no_internal_overlap(k);
   at::assert_no_overlap(q, k);
