@@ -100,3 +100,15 @@ def test_pair_product_hands_buffers_and_scales_back(cuda_device, monkeypatch, la
         wrong += (torch_ops.gemm_fp8(a, sa, b, sb, out_dtype=F32) != want).sum()
     torch.cuda.synchronize()
     assert wrong.item() == 0 and _native.device_error() == 0
+
+
+def test_rotary_refuses_more_heads_than_it_counts(cuda_device):
+    """Sizes past 32 bits are refused before the result is allocated, not cut to their low bits."""
+    table, pos = torch.zeros(4, 2, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    one = rand(1, 1, 2, dtype=BF16)
+    for q, k in ((one.expand(1, 2 ** 32 + 2, 2), one), (one, one.expand(1, 2 ** 32 + 2, 2)),
+                 (one.expand(1, 65537, 2), one), (rand(1, 1, 1).expand(1, 1, 65538), rand(1, 1, 1).expand(1, 1, 65538))):
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(RuntimeError, match="at most 65536|contiguous heads"):
+            torch_ops.rotary(q, k, pos, table)
+        assert torch.cuda.memory_allocated() == before
