@@ -118,7 +118,8 @@ int zcutlass_version_minor(void);
 int zcutlass_version_patch(void);
 
 /* Device-side error word of the current device: 0 when clean, otherwise a code
- * (site * 16 + role) written by the first kernel whose bounded wait expired.
+ * (site * 16 + role) written by the first kernel whose bounded wait expired,
+ * or, if none did, by a rotary position beyond its table (site 32).
  * Synchronises the device. `clear` != 0 resets the word to 0 afterwards. */
 int zcutlass_device_error(int clear);
 

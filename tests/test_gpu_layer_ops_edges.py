@@ -112,3 +112,16 @@ def test_rotary_refuses_more_heads_than_it_counts(cuda_device):
         with pytest.raises(RuntimeError, match="at most 65536|contiguous heads"):
             torch_ops.rotary(q, k, pos, table)
         assert torch.cuda.memory_allocated() == before
+
+
+def test_position_beyond_the_table_is_not_an_expired_wait(cuda_device):
+    """It is reported, but apart: a wait that expires later still reports its own code, and kernels that skip
+    their work once a wait has expired do not take the position for one."""
+    table = torch_ops.rotary_table(16, 64, device="cuda")
+    q = rand(4, 3, 64, seed=1)
+    _native.device_error(clear=True)
+    torch_ops.rotary(q, q, torch.tensor([3, 16, 15, 1], device="cuda"), table)
+    assert _native.lib().zcutlass_selftest_bounded_wait(2000) == (15 << 4) | 15
+    assert _native.device_error(clear=False) == (32 << 4) | 1
+    assert _native.device_error(clear=True) == (32 << 4) | 1
+    assert _native.device_error() == 0

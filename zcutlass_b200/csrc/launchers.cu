@@ -23,6 +23,10 @@ namespace zcb {
 // One error word per device (each device loading the library gets its own
 // copy of this variable). Kernels set it when a bounded wait expires.
 __device__ int g_device_error_word = 0;
+// Errors in a call's data (a rotary position beyond its table), which leave every
+// other result valid: apart, so that they neither hide an expired wait nor
+// keep the NVLS reduction, which looks at the word above, from its work.
+__device__ int g_device_data_word = 0;
 
 namespace {
 
@@ -61,6 +65,7 @@ DeviceSlot* current_slot() {
     if (cudaGetSymbolAddress(&word, g_device_error_word) == cudaSuccess) {
       info.error_word = static_cast<int*>(word);
     }
+    if (cudaGetSymbolAddress(&word, g_device_data_word) == cudaSuccess) info.data_word = static_cast<int*>(word);
     slot->info = info;
   });
   return slot;
@@ -949,15 +954,23 @@ cudaError_t launch_repack_gemm(const LaunchArgs& a) {
   return e;
 }
 
-int read_and_clear_error_word(bool clear) {
+namespace {
+// The value of one of the words, cleared if asked; -1 if CUDA failed.
+int read_word(const int& symbol, bool clear) {
   int value = 0;
-  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-  if (cudaMemcpyFromSymbol(&value, g_device_error_word, sizeof(int)) != cudaSuccess) return -1;
+  if (cudaMemcpyFromSymbol(&value, symbol, sizeof(int)) != cudaSuccess) return -1;
   if (clear && value != 0) {
     const int zero = 0;
-    if (cudaMemcpyToSymbol(g_device_error_word, &zero, sizeof(int)) != cudaSuccess) return -1;
+    if (cudaMemcpyToSymbol(symbol, &zero, sizeof(int)) != cudaSuccess) return -1;
   }
   return value;
+}
+}  // namespace
+
+int read_and_clear_error_word(bool clear) {
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
+  const int wait = read_word(g_device_error_word, clear), data = read_word(g_device_data_word, clear);
+  return wait < 0 || data < 0 ? -1 : wait != 0 ? wait : data;
 }
 
 uint64_t launch_count() { return g_launches.load(std::memory_order_relaxed); }
@@ -982,11 +995,11 @@ __global__ void selftest_bounded_wait_kernel(uint64_t timeout_ns, int* error_wor
 int selftest_bounded_wait(uint32_t timeout_us) {
   DeviceSlot* slot = current_slot();
   if (slot == nullptr || slot->info.error_word == nullptr) return -1;
-  if (read_and_clear_error_word(true) < 0) return -1;
+  if (cudaDeviceSynchronize() != cudaSuccess || read_word(g_device_error_word, true) < 0) return -1;
   selftest_bounded_wait_kernel<<<1, 32>>>(static_cast<uint64_t>(timeout_us) * 1000ull, slot->info.error_word);
   g_launches.fetch_add(1, std::memory_order_relaxed);
-  if (cudaGetLastError() != cudaSuccess) return -1;
-  return read_and_clear_error_word(true);
+  if (cudaGetLastError() != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) return -1;
+  return read_word(g_device_error_word, true);
 }
 
 // ---------------------------------------------------------------- decode without allocation

@@ -40,6 +40,7 @@ struct DeviceInfo {
   int sm_count = 0;
   int max_smem_optin = 0;
   int* error_word = nullptr;  // device address of this device's error word
+  int* data_word = nullptr;   // the same for errors in a call's data
 };
 const DeviceInfo* current_device_info();
 // Whether kernels are launched with programmatic stream serialization

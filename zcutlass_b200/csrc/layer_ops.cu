@@ -365,7 +365,7 @@ cudaError_t launch_rotary(const zcutlass_rotary_desc& d, const void* q, void* q_
   p.head_dim = d.head_dim;
   p.rotary_dim = d.rotary_dim;
   p.inverse = d.inverse != 0;
-  p.error_word = info->error_word;
+  p.error_word = info->data_word;
   const cudaStream_t stream = static_cast<cudaStream_t>(d.stream);
   const bool inter = d.interleaved != 0;
   if (d.dtype == ZCUTLASS_F16) return rotary_t<half>(p, inter, stream, info->sm_count);

@@ -59,11 +59,12 @@ class TPGroup:
 def check_device_error() -> None:
     """Raises if a kernel of the library recorded an error on the current
     device since the last check (a bounded wait that gave up: an NVLS barrier
-    whose peers never arrived, or a GEMM pipeline wait; or a rotary position
-    beyond its table). After such an error
-    the outputs of the steps since the last check must not be used: the NVLS
-    reduction skips its work once the error word is set. Reading the word
-    synchronises the device; call it between steps, not inside a capture."""
+    whose peers never arrived, or a GEMM pipeline wait; or, if no wait did, a
+    rotary position beyond its table). After a wait that gave up, the outputs
+    of the steps since the last check must not be used: the NVLS reduction
+    skips its work from then on. A rotary position is an error of its token
+    alone and stops nothing else. Reading the word synchronises the device;
+    call it between steps, not inside a capture."""
     from . import _native
 
     code = _native.device_error(clear=True)
