@@ -61,3 +61,18 @@ def test_rotary_on_cpu_tensors_says_so():
     for call in (torch_ops.rotary, torch_ops.rotary_):
         with pytest.raises(RuntimeError, match="q must be a rank-3 CUDA tensor"):
             call(o["q"], o["q"].clone(), o["pos"], o["table"])
+
+
+def test_layer_with_its_own_linear_refuses_8_bit_weights():
+    """Its function takes tensors; it must not be handed anything else."""
+    from zcutlass_b200 import tp
+
+    def linear(x, w, bias, out):
+        out.copy_(x @ w.t())
+
+    layer = tp.TPDecoderLinears(tp.LayerShape(64, 128, 4, 2, 16), tp.TPGroup(), "cpu", torch.float32, linear_fn=linear)
+    x = torch.randn(5, 64)
+    y = layer.forward(x).clone()
+    with pytest.raises(ValueError, match="linear_fn"):
+        layer.quantize_fp8()
+    assert torch.equal(layer.forward(x), y)  # nothing was replaced

@@ -478,8 +478,12 @@ class TPDecoderLinears:
     def quantize_fp8(self) -> None:
         """Replaces the four weights by 8-bit ones (Fp8Weight), half the
         bytes that a decode step reads. The 16-bit weights are dropped;
-        idempotent."""
-        for linear in (self.qkv, self.o_proj, self.gate_up, self.down):
+        idempotent. Refused for a layer with a linear_fn of its own, which
+        takes tensors."""
+        linears = (self.qkv, self.o_proj, self.gate_up, self.down)
+        if any(linear.linear_fn is not _linear_into for linear in linears):
+            raise ValueError("8-bit weights need the library's own linear: this layer was made with a linear_fn")
+        for linear in linears:
             if not isinstance(linear.weight, Fp8Weight):
                 linear.weight = Fp8Weight(linear.weight)
 
