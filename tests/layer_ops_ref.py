@@ -99,3 +99,30 @@ def check_rotated(y, x, positions, table, interleaved, inverse=False):
     size = x.double().abs().amax(-1, keepdim=True) * 2 * max(1.0, table.abs().max().item()) if x.numel() else ref
     bound = half_ulp(ref, y.dtype) + size * (3 * 2.0 ** -24) * (1 + torch.finfo(y.dtype).eps)
     assert ((y.double() - ref).abs() <= bound).all()
+
+
+# ---------------------------------------------------------------- gradients against differences
+
+
+def aligned_signs(m: int, n: int, k: int, seed: int = 0):
+    """x [m, k], w [n, k], c [m, n] in 32 bits, magnitudes in [0.5, 1.5], with signs s_m u_k, t_n u_k and
+    s_m t_n: every term of y = x w^T, of c w and of c^T x has the sign of its sum, so nothing cancels."""
+    g = torch.Generator().manual_seed(seed)
+    s, t, u = (torch.randint(0, 2, (d,), generator=g) * 2.0 - 1.0 for d in (m, n, k))
+    mag = lambda *d: torch.rand(*d, generator=g) + 0.5  # noqa: E731
+    return s[:, None] * u * mag(m, k), t[:, None] * u * mag(n, k), s[:, None] * t * mag(m, n)
+
+
+def difference_error(loss, x, other, c, grad, step: float = 4.0):
+    """(error, bound): the derivative of loss(x) along v = sign(x), by a difference over x +- step v, against
+    sum(grad * v), where loss(x) = sum(c * (Q(x) Q(other)^T)) and grad = Q(c) Q(other). A value a of a group
+    with largest value A is off by at most 2^-4 (|a| + 2^-13 A) (half a step relative to the value, or half the
+    smallest step), a product of two such by e = 2^-3 + 2^-8 of its absolute terms. With aligned_signs both
+    errors are near e times the derivative itself: the bound is about a quarter of it."""
+    v = torch.sign(x)
+    diff = (loss(x + step * v) - loss(x - step * v)) / (2 * step)
+    size = lambda t: t.double().abs() + 2.0 ** -13 * t.double().abs().max()  # noqa: E731
+    e = 2.0 ** -3 + 2.0 ** -8 + 2.0 ** -16  # and the roundings of sums in 32 bits
+    terms = (((size(x + step * v) + size(x - step * v)) @ size(other).t()) * c.double().abs()).sum() / (2 * step)
+    grads = (size(c) @ size(other)).sum()
+    return (diff - (grad.double() * v.double()).sum()).abs().item(), (e * (terms + grads)).item()

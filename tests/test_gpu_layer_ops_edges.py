@@ -125,3 +125,20 @@ def test_position_beyond_the_table_is_not_an_expired_wait(cuda_device):
     assert _native.device_error(clear=False) == (32 << 4) | 1
     assert _native.device_error(clear=True) == (32 << 4) | 1
     assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("mnk", [(64, 96, 128), (130, 200, 260), (300, 512, 640)], ids=str)
+def test_train_gradients_agree_with_differences(cuda_device, mnk):
+    """Of x and of w, in directions in which no term cancels (layer_ops_ref.difference_error: what the bound
+    tells apart is tested on the CPU)."""
+    x, w, c = (t.cuda() for t in R.aligned_signs(*mnk, seed=2))
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    torch_ops.linear_fp8_train(xg, wg).backward(c)
+    of_x = lambda v: (torch_ops.linear_fp8_train(v, w).double() * c.double()).sum()  # noqa: E731
+    of_w = lambda v: (torch_ops.linear_fp8_train(x, v).double() * c.double()).sum()  # noqa: E731
+    for loss, leaf, other, grad, cc in ((of_x, x, w, xg.grad, c), (of_w, w, x, wg.grad, c.t())):
+        error, bound = R.difference_error(loss, leaf, other, cc, grad)
+        assert error <= bound
+        for wrong in (grad * 0, -grad, grad.roll(1, 0), grad.roll(1, 1)):
+            error, bound = R.difference_error(loss, leaf, other, cc, wrong)
+            assert error > bound

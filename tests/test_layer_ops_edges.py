@@ -7,6 +7,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import layer_ops_ref as R
 from zcutlass_b200 import torch_ops
 
 E4M3 = torch.float8_e4m3fn
@@ -76,3 +77,22 @@ def test_layer_with_its_own_linear_refuses_8_bit_weights():
     with pytest.raises(ValueError, match="linear_fn"):
         layer.quantize_fp8()
     assert torch.equal(layer.forward(x), y)  # nothing was replaced
+
+
+def test_difference_bound_tells_wrong_gradients():
+    """The bound that the GPU test of the differentiable linear uses holds for the formulas in 64 bits, and no
+    mistake passes it: no gradient, the wrong sign, rows or columns in another order, half of the sum."""
+    x, w, c = R.aligned_signs(64, 96, 128, seed=1)
+    product = lambda a, b: R.values(*R.quantize(a, E4M3, 1)) @ R.values(*b).t()  # noqa: E731
+    blocks = lambda t: R.quantize(t, E4M3, 128)  # noqa: E731
+    along = lambda t: R.quantize(t, E4M3, 1)  # noqa: E731
+    turned = lambda q: (q[0].t(), q[1].t())  # noqa: E731
+    dx, dw = product(c, turned(blocks(w))), product(c.t(), along(x.t()))
+    of_x = lambda v: (product(v, blocks(w)) * c.double()).sum()  # noqa: E731
+    of_w = lambda v: (product(x, blocks(v)) * c.double()).sum()  # noqa: E731
+    for loss, leaf, other, grad, cc in ((of_x, x, w, dx, c), (of_w, w, x, dw, c.t())):
+        error, bound = R.difference_error(loss, leaf, other, cc, grad)
+        assert error <= bound
+        for wrong in (grad * 0, -grad, grad.roll(1, 0), grad.roll(1, 1), grad * 0.5):
+            error, bound = R.difference_error(loss, leaf, other, cc, wrong)
+            assert error > bound
