@@ -96,3 +96,17 @@ def test_difference_bound_tells_wrong_gradients():
         for wrong in (grad * 0, -grad, grad.roll(1, 0), grad.roll(1, 1), grad * 0.5):
             error, bound = R.difference_error(loss, leaf, other, cc, wrong)
             assert error > bound
+
+
+def test_rotary_head_limit_is_an_error_not_a_crash():
+    """On tensors of CUDA's type without storage: the check comes before any work."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    torch_ops.load()
+    with FakeTensorMode():
+        one = torch.empty(1, 1, 2, device="cuda")
+        pos, table = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.empty(4, 2, device="cuda")
+        for heads in (65537, 2 ** 32 + 2):
+            for q, k in ((one.expand(1, heads, 2), one), (one, one.expand(1, heads, 2))):
+                with pytest.raises(RuntimeError, match="at most 65536"):
+                    torch_ops.rotary(q, k, pos, table)

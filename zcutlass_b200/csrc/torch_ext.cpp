@@ -436,8 +436,7 @@ constexpr int64_t kMaxHeads = 65536;  // and values of a head: what zcutlass_rot
 // The checks of q and k, before anything is allocated or a device is made current.
 void check_heads(const at::Tensor& t, const char* name, const at::Tensor& q) {
   TORCH_CHECK(t.is_cuda() && t.dim() == 3, name, " must be a rank-3 CUDA tensor [tokens, heads, head_dim]");
-  TORCH_CHECK(t.size(1) <= kMaxHeads && t.size(2) <= kMaxHeads, name, " must have at most ", kMaxHeads, " heads of at most ",
-              kMaxHeads, " values");
+  TORCH_CHECK(t.size(1) <= kMaxHeads && t.size(2) <= kMaxHeads, name, " must have at most 65536 heads of at most 65536 values");
   (void)float_code(t, name);
   TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, name, " must have contiguous heads (last dimension)");
   TORCH_CHECK(t.scalar_type() == q.scalar_type() && t.device() == q.device() && t.size(0) == q.size(0) &&
