@@ -142,3 +142,28 @@ def test_train_gradients_agree_with_differences(cuda_device, mnk):
         for wrong in (grad * 0, -grad, grad.roll(1, 0), grad.roll(1, 1)):
             error, bound = R.difference_error(loss, leaf, other, cc, wrong)
             assert error > bound
+
+
+def test_two_streams_of_one_capture_share_a_leaf(cuda_device):
+    w = rand(128, 256, seed=1, dtype=BF16).requires_grad_()
+    x = [rand(40, 256, seed=2 + i, dtype=BF16) for i in (0, 1)]
+    dy = rand(40, 128, seed=4, dtype=BF16)
+    side = torch.cuda.Stream()
+
+    def step():
+        here = torch.cuda.current_stream()
+        y0 = torch_ops.linear_fp8_train(x[0], w)
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            y1 = torch_ops.linear_fp8_train(x[1], w)
+        here.wait_stream(side)
+        return (y0.detach(), y1.detach()) + torch.autograd.grad((y0, y1), w, (dy, dy))
+
+    want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -507,18 +507,31 @@ void check_no_tangent(const char* name, const T&... t) {
   TORCH_CHECK(!((t.defined() && t._fw_grad(0).defined()) || ...), name, " has no forward-mode derivative");
 }
 
-// While the current stream is being captured: refuses a leaf whose gradient accumulator was made on another
-// stream and is still alive (an eager graph of the same leaf is). The backward pass would wait for that
-// stream, which ends the capture, or the process.
-void check_capture(const at::Tensor& leaf) {
-  if (!wants_grad(leaf) || !leaf.is_cuda() || leaf.grad_fn() != nullptr) return;
+// Whether work on `stream` is part of the capture that `id` names (the legacy stream never is).
+bool in_capture(const c10::Stream& stream, unsigned long long id) {
+  const cudaStream_t s = c10::cuda::CUDAStream(stream).stream();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long other = 0;
+  return s != nullptr && cudaStreamGetCaptureInfo(s, &status, &other) == cudaSuccess &&
+         status == cudaStreamCaptureStatusActive && other == id;
+}
+
+// While the current stream is being captured: refuses a leaf whose gradient accumulator
+// was made outside the capture and is still alive (an eager graph of the same leaf is). The backward pass would
+// wait for that accumulator's stream, which ends the capture, or the process.
+void check_capture(const at::Tensor& t) {
+  if (!wants_grad(t) || !t.is_cuda() || t.grad_fn() != nullptr) return;
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
-  if (accumulator == nullptr) return;
-  const auto made_on = accumulator->stream();
-  TORCH_CHECK(!made_on.has_value() || *made_on == at::cuda::getCurrentCUDAStream(leaf.get_device()).unwrap(),
-              "a graph of this leaf made on another stream is still alive: drop it (its outputs and losses) before "
-              "capturing a backward pass");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream(t.get_device()).stream(), &status, &id));
+  const auto check = [id](torch::autograd::Node* accumulator) {
+    const auto made_on = accumulator->stream();
+    TORCH_CHECK(!made_on.has_value() || in_capture(*made_on, id),
+                "a graph of this leaf made on another stream is still alive: drop it (its outputs and losses) before "
+                "capturing a backward pass");
+  };
+  if (const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t)) check(accumulator.get());
 }
 
 template <typename... T>
