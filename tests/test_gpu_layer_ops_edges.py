@@ -144,6 +144,34 @@ def test_train_gradients_agree_with_differences(cuda_device, mnk):
             assert error > bound
 
 
+def test_capture_is_refused_where_an_eager_graph_of_an_upstream_leaf_lives(cuda_device):
+    """Views of a leaf, and what was computed from it, are refused as the leaf itself is."""
+    qkv = rand(32, 8 * 64, seed=1, dtype=BF16).requires_grad_()
+    w = rand(128, 512, seed=2, dtype=BF16).requires_grad_()
+    table, pos = torch_ops.rotary_table(32, 64, device="cuda"), torch.arange(32, device="cuda")
+    dy = rand(32, 6, 64, seed=3, dtype=BF16)
+
+    def turn():
+        q, _ = torch_ops.rotary(qkv[:, :384].unflatten(1, (6, 64)), qkv[:, 384:].unflatten(1, (2, 64)), pos, table)
+        return torch.autograd.grad(q, qkv, dy)
+
+    def project():
+        return torch_ops.linear_fp8_train(qkv * 2, w)
+
+    want = turn()[0].clone()
+    eager = qkv * 3  # any graph of the leaf
+    for step in (turn, project):
+        with pytest.raises(RuntimeError, match="before capturing"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                step()
+    del eager
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = turn()[0]
+    g.replay()
+    assert torch.equal(got, want)
+
+
 def test_two_streams_of_one_capture_share_a_leaf(cuda_device):
     w = rand(128, 256, seed=1, dtype=BF16).requires_grad_()
     x = [rand(40, 256, seed=2 + i, dtype=BF16) for i in (0, 1)]

@@ -23,12 +23,14 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <optional>
 #include <string_view>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "zcutlass/gemm.hpp"
@@ -516,11 +518,11 @@ bool in_capture(const c10::Stream& stream, unsigned long long id) {
          status == cudaStreamCaptureStatusActive && other == id;
 }
 
-// While the current stream is being captured: refuses a leaf whose gradient accumulator
+// While the current stream is being captured: refuses an operand that leads to a leaf whose gradient accumulator
 // was made outside the capture and is still alive (an eager graph of the same leaf is). The backward pass would
 // wait for that accumulator's stream, which ends the capture, or the process.
 void check_capture(const at::Tensor& t) {
-  if (!wants_grad(t) || !t.is_cuda() || t.grad_fn() != nullptr) return;
+  if (!wants_grad(t) || !t.is_cuda()) return;
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long id = 0;
@@ -531,7 +533,19 @@ void check_capture(const at::Tensor& t) {
                 "a graph of this leaf made on another stream is still alive: drop it (its outputs and losses) before "
                 "capturing a backward pass");
   };
-  if (const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t)) check(accumulator.get());
+  if (t.grad_fn() == nullptr) {
+    if (const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t)) check(accumulator.get());
+    return;
+  }
+  std::vector<torch::autograd::Node*> left{t.grad_fn().get()};
+  std::unordered_set<torch::autograd::Node*> seen(left.begin(), left.end());
+  while (!left.empty()) {
+    torch::autograd::Node* node = left.back();
+    left.pop_back();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node) != nullptr) check(node);
+    for (const auto& edge : node->next_edges())
+      if (edge.is_valid() && seen.insert(edge.function.get()).second) left.push_back(edge.function.get());
+  }
 }
 
 template <typename... T>
