@@ -107,7 +107,7 @@ __device__ __forceinline__ void load_row_chunk(const T* src, int valid, float (&
     const uint4* v = reinterpret_cast<const uint4*>(src);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint4 u = __ldg(v + j);
+      const uint4 u = ld_written(v + j);
       const float2 f0 = Elem<T>::unpack(u.x), f1 = Elem<T>::unpack(u.y);
       const float2 f2 = Elem<T>::unpack(u.z), f3 = Elem<T>::unpack(u.w);
       out[8 * j + 0] = f0.x; out[8 * j + 1] = f0.y; out[8 * j + 2] = f1.x; out[8 * j + 3] = f1.y;
