@@ -195,3 +195,13 @@ def test_two_streams_of_one_capture_share_a_leaf(cuda_device):
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("k", [300, 768, 896, 1280, 1536, 1792, 2560])
+@pytest.mark.parametrize("m", [1, 16, 20, 64])
+def test_short_products_of_few_rows(cuda_device, m, k):
+    """K of few blocks: every count of splits that the choice can come to, over few and many tiles."""
+    for n in (1, 256, 1000, 2048, 4096):
+        a, sa = torch_ops.quantize_fp8(rand(m, k, seed=m))
+        b, sb = torch_ops.quantize_fp8(rand(n, k, seed=n), layout="blocks")
+        R.check_product(torch_ops.gemm_fp8(a, sa, b, sb, out_dtype=F32), *R.product(a, sa, b, sb), k)

@@ -228,8 +228,11 @@ int resident_clusters(const DeviceInfo& dev, int size) {
 // CTAs along K per tile, each with at least two blocks, at most a cluster of 8. The swapped kernel, two CTAs
 // of which fit an SM: the power of two that gives (nearly) every SM one, since more only add partial tiles to
 // exchange, and clusters of other sizes leave SMs out: 16 x 4096 x 4096 (32 tiles) takes 8.3, 6.5 and 7.6 us
-// with 2, 4 and 8 splits, 1 x 6144 x 4096 (48 tiles) 8.6, 8.4, 7.4, 8.5 and 12.1 with 2, 3, 4, 5 and 6. The
-// other, one CTA of which fills an SM: as many as run at once (200 x 1024 x 4096, 16 tiles: 13.3 us with 8
+// with 2, 4 and 8 splits, 1 x 6144 x 4096 (48 tiles) 8.6, 8.4, 7.4, 8.5 and 12.1 with 2, 3, 4, 5 and 6. Where a
+// short K ends below the next power of two, all that it gives (3, 5 or 6) while that is no more than about 60
+// CTAs: 1 x 256 x 1536 (2 tiles) takes 3.5 us with 4 splits and 3.1 with 6, 1 x 1536 x 1280 (12 tiles) 3.8 with 4
+// and 3.7 with 5, but 1 x 2048 x 1536 (16 tiles) 3.9 with 4 and 4.1 with 6, 1 x 1024 x 1792 4.0 with 4, 4.2 with 7.
+// The other, one CTA of which fills an SM: as many as run at once (200 x 1024 x 4096, 16 tiles: 13.3 us with 8
 // splits in two waves).
 int tile_splits(int64_t tiles, int64_t num_kb, const DeviceInfo& dev, bool swap) {
   const char* v = std::getenv("ZCUTLASS_SPLITK");
@@ -238,7 +241,8 @@ int tile_splits(int64_t tiles, int64_t num_kb, const DeviceInfo& dev, bool swap)
   if (v != nullptr && v[0] != '\0') {
     s = std::atoi(v);
   } else if (swap) {
-    while (s < most && s * tiles < dev.sm_count * 6 / 7) s *= 2;
+    while (2 * s <= most && s * tiles < dev.sm_count * 6 / 7) s *= 2;
+    if (2 * s > most && most < 7 && most * tiles <= dev.sm_count * 3 / 7) s = most;
   } else {
     for (s = most; s > 1 && tiles > resident_clusters(dev, s); --s) {}
   }
