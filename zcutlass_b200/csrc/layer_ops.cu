@@ -232,9 +232,12 @@ int resident_clusters(const DeviceInfo& dev, int size) {
 // short K ends below the next power of two, all that it gives (3, 5 or 6) while that is no more than about 60
 // CTAs: 1 x 256 x 1536 (2 tiles) takes 3.5 us with 4 splits and 3.1 with 6, 1 x 1536 x 1280 (12 tiles) 3.8 with 4
 // and 3.7 with 5, but 1 x 2048 x 1536 (16 tiles) 3.9 with 4 and 4.1 with 6, 1 x 1024 x 1792 4.0 with 4, 4.2 with 7.
-// The other, one CTA of which fills an SM: as many as run at once (200 x 1024 x 4096, 16 tiles: 13.3 us with 8
+// 32 and 64 rows get a ring that fills the SM where that is a CTA each (see tensor_fp8): then no more clusters than
+// run at once (32 x 2048 x 4096, 16 tiles: 10.1 us with 8 splits, 15 of whose clusters fit, 6.0 with 4; 64 rows
+// 12.4 and 7.2).
+// The other kernel, one CTA of which fills an SM: as many as run at once (200 x 1024 x 4096, 16 tiles: 13.3 us with 8
 // splits in two waves).
-int tile_splits(int64_t tiles, int64_t num_kb, const DeviceInfo& dev, bool swap) {
+int tile_splits(int64_t tiles, int64_t num_kb, const DeviceInfo& dev, bool swap, bool two_per_sm) {
   const char* v = std::getenv("ZCUTLASS_SPLITK");
   const int most = static_cast<int>(std::min<int64_t>(fp8_tile::kMaxSplits, num_kb / 2));
   int s = 1;
@@ -243,6 +246,9 @@ int tile_splits(int64_t tiles, int64_t num_kb, const DeviceInfo& dev, bool swap)
   } else if (swap) {
     while (2 * s <= most && s * tiles < dev.sm_count * 6 / 7) s *= 2;
     if (2 * s > most && most < 7 && most * tiles <= dev.sm_count * 3 / 7) s = most;
+    if (!two_per_sm) {
+      while (s > 1 && s * tiles <= dev.sm_count * 7 / 8 && tiles > resident_clusters(dev, s)) s /= 2;
+    }
   } else {
     for (s = most; s > 1 && tiles > resident_clusters(dev, s); --s) {}
   }
@@ -252,7 +258,7 @@ int tile_splits(int64_t tiles, int64_t num_kb, const DeviceInfo& dev, bool swap)
 cudaError_t tensor_fp8(const Fp8GemmParams& g, const Fp8Types& t, const DeviceInfo& dev, cudaStream_t stream) {
   const int64_t tiles_n = div_up(g.n, 128), kb = div_up(g.k, fp8::kBlockK), sms = dev.sm_count;
   const bool any = any_forced();
-  const auto splits = [&](int tm) { return tile_splits(tiles_n * div_up(g.m, tm), kb, dev, tm < 128); };
+  const auto splits = [&](int tm) { return tile_splits(tiles_n * div_up(g.m, tm), kb, dev, tm < 128, tm == 16); };
   // Where there is no more than a CTA per SM, one with two blocks per stage and the SM's whole shared memory
   // streams faster than one made for two per SM (48 x 4096 x 14336: 15.6 against 17.1 us; with 224 CTAs,
   // 64 x 28672 x 4096, 30.8 against 23.2). 16 rows are served by the same ring both ways.
