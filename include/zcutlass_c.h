@@ -208,9 +208,11 @@ int zcutlass_sum_rows(const float* part, int64_t rows, int64_t cols, void* out, 
  * (elements); each is E4M3 or E5M2, D and bias F16, BF16 or F32. a_scale has
  * an entry per row of A and block; b_scale per row of B (b_scale_rows = 1) or
  * per 128 rows of B (b_scale_rows = 128); scales are any 32-bit values and
- * have element strides *_row, *_blk. Operands at 16-byte aligned addresses
- * with row strides that are multiples of 16 run on the tcgen05 kernels,
- * others on a slower predicated kernel. m = 0 or n = 0 succeeds without
+ * have element strides *_row, *_blk. The product of two scales is formed in
+ * 32 bits: where it leaves their range, the result is infinite, NaN or 0.
+ * Operands at 16-byte aligned addresses with row strides that are multiples of
+ * 16 run on the tcgen05 kernels, others on the CUDA cores, which takes about
+ * 100 times as long for large products. m = 0 or n = 0 succeeds without
  * writes; k = 0 gives D = bias (or 0). Nothing is allocated. */
 typedef struct zcutlass_fp8_gemm_desc {
   int64_t m, n, k;
@@ -236,8 +238,8 @@ int zcutlass_gemm_fp8(const zcutlass_fp8_gemm_desc* desc, const void* A, const f
  * head are copied. Row p of `table` (row stride table_ld >= rotary_dim) holds
  * the rotary_dim / 2 cosines and then the sines of position p, for p in
  * [0, table_rows). A negative position marks padding: its heads are copied as
- * they are. A position >= table_rows does the same and sets the device error
- * word (zcutlass_device_error), site 32.
+ * they are. A position >= table_rows does the same and is reported by
+ * zcutlass_device_error (site 32) where no bounded wait expired.
  * Strides of tokens and heads are in elements, values of a head contiguous;
  * out may equal in (in place), and must not overlap it otherwise. k_heads = 0:
  * q only. positions: int32 (positions64 = 0) or int64. */

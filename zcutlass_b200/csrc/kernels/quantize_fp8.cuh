@@ -212,6 +212,9 @@ __device__ __forceinline__ uint32_t mag_bits(uint32_t m) {
 // transposed bytes go through shared memory to be written as whole 128-byte rows; their 16-byte units are
 // permuted by the column's eighth, so that the 16 threads of a row (8 columns apart) meet different banks.
 // kBlock: one scale for the tile; else one per row (kRows) and one per column (kCols) of it.
+// Four blocks per SM leave 64 registers: both axes of 16-bit values spill 72 bytes per thread and are faster for it
+// (8192 x 4096 bf16 28.5 us against 29.5 with three blocks); blocks with the transpose, at three, spill 12
+// (26.1 us, 5.1 TB/s).
 template <typename T, int kTop, bool kRows, bool kCols, bool kBlock>
 __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 4 ? 2 : (kBlock && kRows && kCols ? 3 : 4))
     tile_kernel(const QuantizeParams p, bool vec_in, bool vec_q, bool vec_qt) {

@@ -26,8 +26,8 @@
 //  - the arrival at the leader's `tmem_empty` hands back TMEM alone, so it is
 //    not a release of memory to the cluster.
 //
-// Measured (random bits, 20 in a row): 8192 x 9472 x 4096 266 us, 2387 TFLOP/s;
-// with a scale per row of B 344 us, 1848 TFLOP/s.
+// Measured (random bits, 20 in a row): 8192 x 9472 x 4096 254 us, 2500 TFLOP/s;
+// with a scale per row of B 334 us, 1900 TFLOP/s.
 //
 // With 128 x 128 weight scales the factor is one product per thread and block.
 // With a scale per row of B (kRows) TMEM is read as 16 x 8 fragments, in which

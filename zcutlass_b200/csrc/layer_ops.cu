@@ -234,7 +234,7 @@ int resident_clusters(const DeviceInfo& dev, int size) {
 // and 3.7 with 5, but 1 x 2048 x 1536 (16 tiles) 3.9 with 4 and 4.1 with 6, 1 x 1024 x 1792 4.0 with 4, 4.2 with 7.
 // 32 and 64 rows get a ring that fills the SM where that is a CTA each (see tensor_fp8): then no more clusters than
 // run at once (32 x 2048 x 4096, 16 tiles: 10.1 us with 8 splits, 15 of whose clusters fit, 6.0 with 4; 64 rows
-// 12.4 and 7.2).
+// 12.4 and 7.2). ZCUTLASS_SPLITK=<s> fixes the count, as it does for the 16-bit split-K kernels.
 // The other kernel, one CTA of which fills an SM: as many as run at once (200 x 1024 x 4096, 16 tiles: 13.3 us with 8
 // splits in two waves).
 int tile_splits(int64_t tiles, int64_t num_kb, const DeviceInfo& dev, bool swap, bool two_per_sm) {

@@ -175,7 +175,10 @@ def gemm_fp8(a, a_scale, b, b_scale, bias=None, out_dtype=None):
 
     a_scale [M, ceil(K / 128)]; b_scale [N, ceil(K / 128)], or
     [ceil(N / 128), ceil(K / 128)] for weights in 128 x 128 blocks: float32 of
-    any value and any strides."""
+    any value and any strides (a product of two scales beyond 32 bits gives an
+    infinity, NaN or 0). Rows whose stride is no multiple of 16 bytes, as
+    .contiguous() leaves them where K is none, run without the tensor cores:
+    about 100 times slower for large products."""
     return _op("gemm_fp8")(a, a_scale, b, b_scale, bias, out_dtype)
 
 
@@ -183,7 +186,9 @@ def linear_fp8(x, weight, weight_scale, bias=None):
     """x [..., K] @ weight [N, K].T (+ bias) with the weight held in 8 bits
     (quantize_fp8(w, "blocks"), or a checkpoint's values and scales) and x
     quantised by rows on the way in; y has x's dtype. For serving; training
-    uses linear_fp8_train."""
+    uses linear_fp8_train. Faster than the 16-bit linear for fewer than about
+    128 rows of x and for more than 512, slower in between (251 x 8960 x 1536:
+    13.3 us against 11.1; 512 x 4096 x 4096: 20.8 against 20.3)."""
     return _op("linear_fp8")(x, weight, weight_scale, bias)
 
 

@@ -477,8 +477,9 @@ class TPDecoderLinears:
 
     def quantize_fp8(self) -> None:
         """Replaces the four weights by 8-bit ones (Fp8Weight), half the
-        bytes that a decode step reads. The 16-bit weights are dropped;
-        idempotent. Refused for a layer with a linear_fn of its own, which
+        bytes that a decode step reads. The 16-bit weights are dropped, also
+        for steps of 128 to 512 rows, which they take slightly less time for
+        (torch_ops.linear_fp8); idempotent. Refused for a layer with a linear_fn of its own, which
         takes tensors."""
         linears = (self.qkv, self.o_proj, self.gate_up, self.down)
         if any(linear.linear_fn is not _linear_into for linear in linears):
